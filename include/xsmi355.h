@@ -459,6 +459,32 @@ int xsmi_softmax_ce_fwd(const float *logits, const int64_t *labels, float *sm, f
 int xsmi_softmax_ce_bwd(const float *sm, const int64_t *labels, const float *upstream, float *dlogits, int M, int N,
                         float scale);
 
+/* ---- optimizer: AdamW over many tensors ------------------------------------------------------------------------
+ *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
+ *   p' = p (1 - lr weight_decay) - lr m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps)
+ * for `count` tensors: ps[i] and gs[i] are ns[i] floats at any element's alignment, their moments the elements from
+ * starts[i] on (a multiple of 256) of the arrays m and v, which hold `moments` elements (a multiple of 256, aligned to 16
+ * bytes) and start as zeros.  Two tensors must not share parameters or moments.  `state` (XSMI_ADAMW_STATE_BYTES bytes of device
+ * memory, zeros at first) holds the count of steps t, which every call moves on, also one that is replayed from a step
+ * graph; lr, the betas and the other scalars of a recorded call are those of the recording.
+ * state_bits 32: m and v are floats, m_exp and v_exp NULL.
+ * state_bits 8: m and v are bytes, m_exp and v_exp an exponent byte E for each 256 elements, that of the block's
+ * largest value, at least 48 (m) and 64 (v).  A byte of m is a sign and a code k of seven bits, of v a code of eight;
+ * k > 0 stands for the float whose bits are (k - 1 + 8 (E - D)) << 20, D = 14 for m and 30 for v, and 0 for zero: three
+ * bits of fraction, fifteen and thirty-one powers of two below the block's largest value.  E = 255: the block held a value of 2^127 or
+ * more, an infinity or NaN, and reads as NaN.  Rounding is stochastic: to a value's bits (noise << 4) + 8 is added and
+ * the lower 20 are dropped, a value below the smallest code becomes that code where it exceeds (noise + 0.5) / 65536 of it; noise is the
+ * lower (m) or upper (v) half of a hash of the element's place in m, of t and of `seed` (mix() of csrc/adamw.hip).  The
+ * parameters are updated from the moments as they are before that rounding.
+ * xsmi_adamw_moments writes the values that 8-bit moments stand for.
+ * The reference has no working optimizer but SGD (xs/optim/sgd.py:4-9). */
+#define XSMI_ADAMW_STATE_BYTES 24
+int xsmi_adamw_step(int count, float *const *ps, const float *const *gs, const size_t *starts, const size_t *ns, void *m, void *v,
+                    uint8_t *m_exp, uint8_t *v_exp, size_t moments, int state_bits, double lr, double beta1, double beta2, double eps,
+                    double weight_decay, uint32_t seed, void *state);
+int xsmi_adamw_moments(const uint8_t *m8, const uint8_t *v8, const uint8_t *m_exp, const uint8_t *v_exp, float *m, float *v,
+                       size_t moments);
+
 #ifdef __cplusplus
 }
 #endif

@@ -372,6 +372,19 @@ class DeviceArray:
         return "DeviceArray(shape=%s, dtype=%s)" % (self.shape, self.dtype)
 
 
+def hand_out(written, read):
+    """What ``ptr`` of the arrays in ``written`` and ``read_ptr`` of those in ``read`` do, for a call that has their
+    addresses in a table already."""
+    graph = _CAPTURE[0]
+    for arrays, change in ((written, 1), (read, 0)):
+        for a in arrays:
+            blk = a._block
+            if graph is None and not blk.lazy_zero and blk.unwritten is None and (blk.cl is None or not blk.cl.valid):
+                blk.version += change
+            else:
+                a.ptr if change else a.read_ptr
+
+
 def empty(shape, dtype=np.float32):
     return DeviceArray(shape, dtype)
 

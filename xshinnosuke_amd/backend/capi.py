@@ -112,6 +112,8 @@ SIGNATURES = {
     "xsmi_softmax_ce_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i]),
     "xsmi_softmax_ce_bwd": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f]),
     "xsmi_fill": (_i, [_vp, _f, _sz]),
+    "xsmi_adamw_step": (_i, [_i] + [_vp] * 8 + [_sz, _i] + [_c.c_double] * 5 + [_c.c_uint32, _vp]),
+    "xsmi_adamw_moments": (_i, [_vp] * 6 + [_sz]),
     "xsmi_graph_begin": (_i, []),
     "xsmi_graph_end": (_i, [_c.POINTER(_vp), _i]),
     "xsmi_graph_launch": (_i, [_vp]),

@@ -846,3 +846,23 @@ def full(shape, value):
     out = empty(shape)
     lib.call("xsmi_fill", out.ptr, float(value), out.size)
     return out
+
+
+# ---- AdamW -----------------------------------------------------------------------------------------------------
+def adamw_step(launch, moments, opt):
+    """One step of ``optim.AdamW`` over the tensors of ``launch`` (its tables of addresses, which belong to arrays that it
+    keeps alive; they are handed out here)."""
+    _array.hand_out(launch.values, launch.grads)
+    m = moments
+    lib.call("xsmi_adamw_step", launch.count, launch.pp, launch.gp, launch.starts, launch.ns, m.m.ptr, m.v.ptr,
+             m.me.ptr if m.me is not None else None, m.ve.ptr if m.ve is not None else None, m.m.size, m.bits,
+             float(opt.lr), float(opt.betas[0]), float(opt.betas[1]), float(opt.epsilon), float(opt.weight_decay), opt.seed, m.state.ptr)
+
+
+def adamw_moments(m8, v8, me, ve):
+    """(m, v) as float32 arrays from their 8-bit form."""
+    if not m8.size == v8.size == 256 * me.size == 256 * ve.size:
+        raise ValueError("adamw_moments: %d and %d codes, %d and %d exponents" % (m8.size, v8.size, me.size, ve.size))
+    m, v = empty((m8.size,)), empty((m8.size,))
+    lib.call("xsmi_adamw_moments", m8.read_ptr, v8.read_ptr, me.read_ptr, ve.read_ptr, m.ptr, v.ptr, m8.size)
+    return m, v

@@ -7,6 +7,7 @@ either a ``numpy.ndarray`` (host) or a :class:`DeviceArray` (MI355X HBM); the
 static graph re-uses one preallocated buffer for a shorter last batch
 (xs/layers/base.py:88-104).
 """
+import itertools
 import weakref
 
 import numpy as np
@@ -379,7 +380,10 @@ class Tensor(object):
 
 
 class Parameter(Tensor):
-    """A trainable leaf (reference xs/core/base.py:360-371)."""
+    """A trainable leaf (reference xs/core/base.py:360-371).  ``serial`` counts parameters as they are made: sets of them
+    can be walked in an order that repeats."""
+
+    _serials = itertools.count(1)
 
     def __new__(cls, *args, **kwargs):
         if len(args) and isinstance(args[0], Parameter):
@@ -389,6 +393,7 @@ class Parameter(Tensor):
     def __init__(self, t=None, **kwargs):
         if isinstance(t, Parameter):
             return
+        self.serial = next(Parameter._serials)
         if isinstance(t, Tensor):
             Tensor.__init__(self, t._data, t.requires_grad, None, t.name, **kwargs)
         else:

@@ -1,0 +1,308 @@
+// AdamW over many tensors in one launch, with moments in 32 or in 8 bits.
+//
+//   m' = beta1 m + (1 - beta1) g        v' = beta2 v + (1 - beta2) g^2
+//   p' = p (1 - lr decay) - lr m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps)
+//
+// The number of steps taken lives in device memory and a one-thread launch in front of the step moves it: a recorded
+// step that is replayed goes on counting.
+//
+// Moments in 8 bits.  Blocks of 256 elements share the exponent byte E of their largest value; a code keeps a float's
+// exponent, counted from E - D, and the three leading bits of its fraction: code k > 0 is the float whose bits are
+// (k - 1 + 8 (E - D)) << 20, and 0 is zero.  The first moment has a sign and seven bits (D = 14), the second eight bits
+// (D = 30).  The scale of a block is a power of two, so a block whose largest value changes keeps its other values
+// where they are: nothing is rounded again that has not moved.  Rounding is stochastic.  To the nearest code it would
+// lose every change below half a step, 3 to 6 % of the value, and the second moment moves by 0.1 % of its distance to
+// g^2 in a step: it would never decay.  The noise is a hash of the element's position, the step and a seed, so a step
+// gives the same bits however it is launched.  The parameters are updated from the moments before they are rounded.
+#include "xsmi_internal.h"
+#include <math.h>
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef f4 f4u __attribute__((aligned(4)));              // parameters and gradients may start at any element
+constexpr int MAX_TENSORS = 96;                          // of one launch: its arguments stay below 4 KB
+constexpr int BLOCK = 256;                               // elements that share an exponent
+
+// What a step needs beside its tensors, moved by the launch in front of it (device memory of the caller).
+struct StepState {
+    uint64_t steps;      // taken so far
+    float rate, root;    // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
+    uint32_t key, unused;
+};
+static_assert(sizeof(StepState) == XSMI_ADAMW_STATE_BYTES, "the header's size of the step state");
+
+struct Tensors {
+    float *p[MAX_TENSORS];
+    const float *g[MAX_TENSORS];
+    uint64_t start[MAX_TENSORS], n[MAX_TENSORS];
+    uint32_t first[MAX_TENSORS];                         // workgroup that a tensor starts with
+    int count;
+};
+
+struct Factors {
+    float keep, b1, c1, b2, c2, eps;                     // 1 - lr decay, beta1, 1 - beta1, beta2, 1 - beta2, eps
+};
+
+struct Moments8 {
+    uint8_t *m, *v, *me, *ve;
+};
+
+constexpr uint32_t STRIDE = 0x9E3779B1u;                 // fraction of the golden ratio, odd
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t h) {
+    h ^= h >> 16;
+    h *= 0x6A09E667u;                                    // fraction of the root of 2
+    h ^= h >> 15;
+    h *= 0xBB67AE85u;                                    // fraction of the root of 3
+    return h ^ (h >> 16);
+}
+
+__device__ double power(double b, uint64_t t) {
+    double r = 1.0;
+    for (; t; t >>= 1, b *= b)
+        if (t & 1) r *= b;
+    return r;
+}
+
+__global__ void adamw_tick_kernel(StepState *s, double lr, double beta1, double beta2, uint32_t seed) {
+    const uint64_t t = s->steps + 1;
+    s->steps = t;
+    s->rate = (float)(lr / (1.0 - power(beta1, t)));
+    s->root = (float)(1.0 / sqrt(1.0 - power(beta2, t)));
+    s->key = mix(seed + (uint32_t)t * STRIDE);
+}
+
+// Each product and sum is rounded by itself: the 8-bit codes are defined by these values of the moments.
+__device__ __forceinline__ void update(float &p, float g, float &m, float &v, const Factors &f, float rate, float root) {
+#pragma clang fp contract(off)
+    m = m * f.b1 + g * f.c1;
+    v = v * f.b2 + g * f.c2 * g;
+    p = p * f.keep - m * rate / (sqrtf(v) * root + f.eps);
+}
+
+// The tensor of this workgroup (the last one whose first workgroup is not behind it).
+__device__ __forceinline__ int tensor_of(const Tensors &t, uint32_t group) {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.first[mid] <= group) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ f4 load4(const float *p, uint64_t i, uint64_t n) {
+    if (i + 4 <= n) return *reinterpret_cast<const f4u *>(p + i);
+    f4 r = {0.f, 0.f, 0.f, 0.f};
+    if (i < n) r.x = p[i];
+    if (i + 1 < n) r.y = p[i + 1];
+    if (i + 2 < n) r.z = p[i + 2];
+    return r;
+}
+
+__device__ __forceinline__ void store4(float *p, uint64_t i, uint64_t n, f4 v) {
+    if (i + 4 <= n) {
+        *reinterpret_cast<f4u *>(p + i) = v;
+        return;
+    }
+    if (i < n) p[i] = v.x;
+    if (i + 1 < n) p[i + 1] = v.y;
+    if (i + 2 < n) p[i + 2] = v.z;
+}
+
+// 256 threads, ITER * 1024 elements of one tensor.  The moments are padded to whole blocks of 256 elements, of which those
+// behind the tensor stay zero: zero gradients of zero moments.
+template <int ITER>
+__global__ void __launch_bounds__(256) adamw_kernel(Tensors t, float *__restrict__ m, float *__restrict__ v, Factors f,
+                                                    const StepState *__restrict__ s) {
+    const int k = tensor_of(t, blockIdx.x);
+    const uint64_t n = t.n[k], base = (uint64_t)(blockIdx.x - t.first[k]) * (1024u * ITER) + 4u * threadIdx.x;
+    float *const p = t.p[k];
+    const float *const g = t.g[k];
+    m += t.start[k];
+    v += t.start[k];
+    const float rate = s->rate, root = s->root;
+    f4 pp[ITER], gg[ITER], mm[ITER], vv[ITER];
+#pragma unroll
+    for (int u = 0; u < ITER; ++u) {
+        const uint64_t i = base + 1024u * u;
+        if (i < n) {
+            pp[u] = load4(p, i, n);
+            gg[u] = load4(g, i, n);
+            mm[u] = *reinterpret_cast<const f4 *>(m + i);
+            vv[u] = *reinterpret_cast<const f4 *>(v + i);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < ITER; ++u) {
+        const uint64_t i = base + 1024u * u;
+        if (i < n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float pe = pp[u][e], me = mm[u][e], ve = vv[u][e];
+                update(pe, gg[u][e], me, ve, f, rate, root);
+                pp[u][e] = pe, mm[u][e] = me, vv[u][e] = ve;
+            }
+            store4(p, i, n, pp[u]);
+            *reinterpret_cast<f4 *>(m + i) = mm[u];
+            *reinterpret_cast<f4 *>(v + i) = vv[u];
+        }
+    }
+}
+
+__device__ __forceinline__ float decode_bits(uint32_t k, int lowest) {       // lowest = 8 (E - D) - 1
+    return __uint_as_float(k ? (uint32_t)((int)k + lowest) << 20 : 0u);
+}
+
+// The code of a non-negative value; noise is 16 bits.  Below the smallest code the choice is between it and zero.
+__device__ __forceinline__ uint32_t encode_bits(uint32_t bits, uint32_t noise, int lowest, float threshold_unit) {
+    const uint32_t k = (uint32_t)((int)((bits + (noise << 4) + 8u) >> 20) - lowest);
+    const uint32_t low = __uint_as_float(bits) > ((float)noise + 0.5f) * threshold_unit ? 1u : 0u;
+    return bits < (uint32_t)(lowest + 1) << 20 ? low : k;
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    return v;
+}
+
+constexpr int DEPTH_M = 14, DEPTH_V = 30, LEAST_M = 48, LEAST_V = 64, BAD = 255;
+
+// One wave of four elements a lane for each block of 256.
+template <int ITER>
+__global__ void __launch_bounds__(256) adamw8_kernel(Tensors t, Moments8 q, Factors f, const StepState *__restrict__ s) {
+    const int k = tensor_of(t, blockIdx.x);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t n = t.n[k], base = (uint64_t)(blockIdx.x - t.first[k]) * (1024u * ITER) + 256u * wave;
+    const float *const g = t.g[k];
+    float *const p = t.p[k];
+    const float rate = s->rate, root = s->root;
+    const uint32_t key = s->key;
+#pragma unroll
+    for (int u = 0; u < ITER; ++u) {
+        const uint64_t block = base + 1024u * u, i = block + 4u * lane;
+        if (block >= n) break;                           // the same for the whole wave
+        const uint64_t at = t.start[k] + i;
+        f4 pp = load4(p, i, n);
+        const f4 gg = load4(g, i, n);
+        uint32_t mq = *reinterpret_cast<const uint32_t *>(q.m + at), vq = *reinterpret_cast<const uint32_t *>(q.v + at);
+        const uint64_t b = (t.start[k] + block) / BLOCK;
+        int em = q.me[b], ev = q.ve[b];
+        const int lm = 8 * (em - DEPTH_M) - 1, lv = 8 * (ev - DEPTH_V) - 1;
+        float mm[4], vv[4];
+        uint32_t mmax = 0, vmax = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t mk = mq >> (8 * e) & 255u, vk = vq >> (8 * e) & 255u;
+            mm[e] = em == BAD ? NAN : copysignf(decode_bits(mk & 127u, lm), __uint_as_float(mk << 24));
+            vv[e] = ev == BAD ? NAN : decode_bits(vk, lv);
+            float pe = pp[e];
+            update(pe, gg[e], mm[e], vv[e], f, rate, root);
+            pp[e] = pe;
+            mmax = max(mmax, __float_as_uint(mm[e]) & 0x7fffffffu);
+            vmax = max(vmax, __float_as_uint(vv[e]) & 0x7fffffffu);
+        }
+        store4(p, i, n, pp);
+        em = max((int)(wave_max(mmax) >> 23), LEAST_M);
+        ev = max((int)(wave_max(vmax) >> 23), LEAST_V);
+        const int lm2 = 8 * (em - DEPTH_M) - 1, lv2 = 8 * (ev - DEPTH_V) - 1;
+        const float um = __uint_as_float((uint32_t)(em - DEPTH_M - 16) << 23), uv = __uint_as_float((uint32_t)(ev - DEPTH_V - 16) << 23);
+        mq = vq = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint64_t pos = at + e;
+            const uint32_t h = mix((uint32_t)pos * STRIDE + key + (uint32_t)(pos >> 32) * 0x510E527Fu);
+            const uint32_t mb = __float_as_uint(mm[e]), vb = __float_as_uint(vv[e]);
+            mq |= (encode_bits(mb & 0x7fffffffu, h & 0xffffu, lm2, um) | (mm[e] < 0.f ? 128u : 0u)) << (8 * e);
+            vq |= encode_bits(vb, h >> 16, lv2, uv) << (8 * e);
+        }
+        // A value of 2^127 and more, an infinity or NaN: the whole block reads as NaN from now on.
+        if (em >= 254) em = BAD, mq = 0;
+        if (ev >= 254) ev = BAD, vq = 0;
+        *reinterpret_cast<uint32_t *>(q.m + at) = mq;
+        *reinterpret_cast<uint32_t *>(q.v + at) = vq;
+        if (lane == 0) q.me[b] = (uint8_t)em, q.ve[b] = (uint8_t)ev;
+    }
+}
+
+// The values that 8-bit moments stand for, four of each a thread.
+__global__ void __launch_bounds__(256) adamw_moments_kernel(Moments8 q, float *__restrict__ m, float *__restrict__ v, uint64_t n) {
+    const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    const uint32_t mq = *reinterpret_cast<const uint32_t *>(q.m + i), vq = *reinterpret_cast<const uint32_t *>(q.v + i);
+    const int em = q.me[i / BLOCK], ev = q.ve[i / BLOCK];
+    f4 mm, vv;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t mk = mq >> (8 * e) & 255u, vk = vq >> (8 * e) & 255u;
+        mm[e] = em == BAD ? NAN : copysignf(decode_bits(mk & 127u, 8 * (em - DEPTH_M) - 1), __uint_as_float(mk << 24));
+        vv[e] = ev == BAD ? NAN : decode_bits(vk, 8 * (ev - DEPTH_V) - 1);
+    }
+    *reinterpret_cast<f4 *>(m + i) = mm;
+    *reinterpret_cast<f4 *>(v + i) = vv;
+}
+
+}  // namespace
+
+extern "C" {
+
+int xsmi_adamw_step(int count, float *const *ps, const float *const *gs, const size_t *starts, const size_t *ns, void *m, void *v,
+                    uint8_t *m_exp, uint8_t *v_exp, size_t moments, int state_bits, double lr, double beta1, double beta2, double eps,
+                    double weight_decay, uint32_t seed, void *state) {
+    XSMI_REQUIRE_INIT();
+    XSMI_CHECK_ARG(count >= 0 && (count == 0 || (ps && gs && starts && ns)), "xsmi_adamw_step: bad argument");
+    XSMI_CHECK_ARG(state_bits == 32 || state_bits == 8, "xsmi_adamw_step: moments in 32 or 8 bits, not %d", state_bits);
+    XSMI_CHECK_ARG(m && v && state && (state_bits == 32 || (m_exp && v_exp)), "xsmi_adamw_step: null pointer");
+    XSMI_CHECK_ARG((((uintptr_t)m | (uintptr_t)v) & 15) == 0 && ((uintptr_t)state & 7) == 0, "xsmi_adamw_step: the moments are not aligned to 16 bytes");
+    XSMI_CHECK_ARG(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "xsmi_adamw_step: betas %g and %g, expected 0 <= beta < 1", beta1, beta2);
+    XSMI_CHECK_ARG(lr >= 0 && eps >= 0 && weight_decay >= 0, "xsmi_adamw_step: negative rate, epsilon or decay");
+    for (int i = 0; i < count; ++i) {
+        XSMI_CHECK_ARG(ps[i] && gs[i], "xsmi_adamw_step: null pointer in tensor %d", i);
+        XSMI_CHECK_ARG(starts[i] % BLOCK == 0 && starts[i] <= moments && ns[i] <= moments - starts[i],
+                       "xsmi_adamw_step: tensor %d has its moments at %zu of %zu", i, starts[i], moments);
+        XSMI_CHECK_ARG(ns[i] < (1ull << 40), "xsmi_adamw_step: tensor %d too large", i);
+    }
+    XSMI_CHECK_ARG(moments % BLOCK == 0, "xsmi_adamw_step: room for %zu moments, expected a multiple of %d", moments, BLOCK);
+    hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(1), 0, xsmi::stream(), (StepState *)state, lr, beta1, beta2, seed);
+    XSMI_LAUNCH_CHECK("adamw_tick_kernel");
+    const Factors f = {(float)(1.0 - lr * weight_decay), (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
+    const Moments8 q = {(uint8_t *)m, (uint8_t *)v, m_exp, v_exp};
+    constexpr int ITER = 4;
+    for (int done = 0; done < count;) {
+        Tensors t;
+        uint64_t groups = 0;
+        int k = 0;
+        for (; done < count && k < MAX_TENSORS; ++done) {
+            if (ns[done] == 0) continue;
+            const uint64_t more = (ns[done] + 1024u * ITER - 1) / (1024u * ITER);
+            if (groups + more > 0x7fffffffull) break;
+            t.p[k] = ps[done], t.g[k] = gs[done], t.start[k] = starts[done], t.n[k] = ns[done];
+            t.first[k++] = (uint32_t)groups;
+            groups += more;
+        }
+        t.count = k;
+        if (k == 0) break;
+        if (state_bits == 32)
+            hipLaunchKernelGGL(adamw_kernel<ITER>, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), t, (float *)m, (float *)v, f, (const StepState *)state);
+        else
+            hipLaunchKernelGGL(adamw8_kernel<ITER>, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), t, q, f, (const StepState *)state);
+        XSMI_LAUNCH_CHECK("adamw_kernel");
+    }
+    return XSMI_OK;
+}
+
+int xsmi_adamw_moments(const uint8_t *m8, const uint8_t *v8, const uint8_t *m_exp, const uint8_t *v_exp, float *m, float *v, size_t moments) {
+    XSMI_REQUIRE_INIT();
+    if (moments == 0) return XSMI_OK;
+    XSMI_CHECK_ARG(m8 && v8 && m_exp && v_exp && m && v, "xsmi_adamw_moments: null pointer");
+    XSMI_CHECK_ARG(moments % BLOCK == 0, "xsmi_adamw_moments: %zu moments, expected a multiple of %d", moments, BLOCK);
+    XSMI_CHECK_ARG((((uintptr_t)m | (uintptr_t)v) & 15) == 0 && (((uintptr_t)m8 | (uintptr_t)v8) & 3) == 0, "xsmi_adamw_moments: unaligned moments");
+    const uint64_t groups = (moments + 1023) / 1024;
+    XSMI_CHECK_ARG(groups < (1ull << 31), "xsmi_adamw_moments: too many moments");
+    const Moments8 q = {(uint8_t *)m8, (uint8_t *)v8, (uint8_t *)m_exp, (uint8_t *)v_exp};
+    hipLaunchKernelGGL(adamw_moments_kernel, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), q, m, v, (uint64_t)moments);
+    XSMI_LAUNCH_CHECK("adamw_moments_kernel");
+    return XSMI_OK;
+}
+
+}  // extern "C"

@@ -1,2 +1,2 @@
 """``xs.nn.optimizers`` is the import path the reference's README uses; the classes live in ``optim``."""
-from ..optim import Optimizer, SGD, get_optimizer  # noqa: F401
+from ..optim import Optimizer, SGD, AdamW, get_optimizer  # noqa: F401

@@ -1,21 +1,8 @@
-"""Optimizers (counterpart of xs/optim).  Only SGD demonstrably works in the reference (the others use an
-undefined ``np``, e.g. xs/optim/sgd.py:21), so only SGD is provided."""
+"""Optimizers (counterpart of xs/optim).  Of the reference's only SGD demonstrably works (the others use an
+undefined ``np``, e.g. xs/optim/sgd.py:21), so only SGD follows it; AdamW is this package's own."""
 from ..nn import array_ops as A
-
-
-class Optimizer:
-    def __init__(self, parameters=None, lr=0.01, weight_decay=0.):
-        self._parameters = parameters
-        self.lr = lr
-        self.weight_decay = weight_decay
-        self.iterations = 0
-
-    def zero_grad(self):
-        for v in self._parameters:
-            v.zero_grad()
-
-    def step(self):
-        self.iterations += 1
+from .base import Optimizer
+from .adamw import AdamW
 
 
 class SGD(Optimizer):
@@ -30,7 +17,9 @@ def get_optimizer(optimizer, **kwargs):
     if isinstance(optimizer, str):
         if optimizer.lower() in ('sgd',):
             return SGD(**kwargs)
-        raise ValueError('unknown optimizer %r (only sgd is available)' % optimizer)
+        if optimizer.lower() in ('adamw',):
+            return AdamW(**kwargs)
+        raise ValueError('unknown optimizer %r (sgd and adamw are available)' % optimizer)
     if isinstance(optimizer, Optimizer):
         if kwargs.get('parameters') is not None:
             optimizer._parameters = kwargs['parameters']
