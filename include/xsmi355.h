@@ -459,6 +459,25 @@ int xsmi_softmax_ce_fwd(const float *logits, const int64_t *labels, float *sm, f
 int xsmi_softmax_ce_bwd(const float *sm, const int64_t *labels, const float *upstream, float *dlogits, int M, int N,
                         float scale);
 
+/* ---- root-mean-square normalisation of rows ------------------------------------------------------------------
+ * s = x + residual, r = 1 / sqrt(mean_j s_j^2 + eps), y_j = gamma_j s_j r over (rows, cols) float32 matrices, rows dense.  residual and sum
+ * (the matrix s) come together or are both NULL (s = x); rstd (rows values r, or NULL) is what the backward
+ * reads.  Sums are in float32: values of 1e19 and above overflow them.
+ * The int8 form stores q_j = round(127 y_j / max_i |y_i|), ties to even, and scale = max_i |y_i| / 127 for each row, with the sums and
+ * the rounding in 64 bits; a row of zeros has the scale 0, one whose y are not all finite the numbers 0 and the scale NaN.
+ * The reference normalises over the batch only (xs/layers/normalize.py:22-56). */
+int xsmi_rms_norm_fwd(const float *x, const float *residual, const float *gamma, float *sum, float *y, float *rstd, size_t rows, int cols,
+                      float eps);
+int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma, float *sum, int8_t *q, float *scale, size_t rows, int cols,
+                       float eps);
+/* With a_j = gamma_j dy_j and xhat_j = s_j r: g_j = ds_j + r (a_j - xhat_j mean_i(a_i xhat_i)), dx1 = beta1 dx1 + g,
+ * dx2 = beta2 dx2 + g, dgamma_j = beta_gamma dgamma_j + sum over rows of dy_j xhat_j; the betas are 0 or 1.  ds (the
+ * gradient that reaches s another way), dx1, dx2 (both addends of s get the same gradient) and dgamma may be NULL; dx1, dx2 and ds may not overlap, but for
+ * dx1 == ds.  The workspace is needed for dgamma; the sums are added in an order that depends on the sizes alone. */
+size_t xsmi_rms_norm_workspace_bytes(size_t rows, int cols);
+int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const float *gamma, const float *ds, float *dx1, float beta1,
+                      float *dx2, float beta2, float *dgamma, float beta_gamma, size_t rows, int cols, void *ws, size_t ws_bytes);
+
 /* ---- optimizer: AdamW over many tensors ------------------------------------------------------------------------
  *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
  *   p' = p (1 - lr weight_decay) - lr m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps)

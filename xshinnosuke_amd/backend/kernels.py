@@ -848,6 +848,67 @@ def full(shape, value):
     return out
 
 
+# ---- root-mean-square normalisation -----------------------------------------------------------------------------
+def _rms_operands(x, gamma, residual):
+    if x.dtype != np.float32 or gamma.dtype != np.float32 or (residual is not None and residual.dtype != np.float32):
+        raise ValueError("rms_norm: operands must be float32")
+    if not x.shape or gamma.size != x.shape[-1]:
+        raise ValueError("rms_norm: %d scales for rows of shape %s" % (gamma.size, x.shape))
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError("rms_norm: residual %s and input %s differ" % (residual.shape, x.shape))
+    cols = x.shape[-1]
+    return (x.size // cols if cols else 0), cols
+
+
+def rms_norm_fwd(x, gamma, eps, residual=None, y=None, want_rstd=True):
+    """(y, s, rstd): y = gamma * s * rstd over rows of the last axis, s = x + residual (x itself without one),
+    rstd = 1 / sqrt(mean(s^2) + eps)."""
+    rows, cols = _rms_operands(x, gamma, residual)
+    y = _like(x, y)
+    if cols == 0:
+        raise ValueError("rms_norm: rows without elements")
+    y.take_fresh()
+    s = empty(x.shape) if residual is not None else x
+    rstd = empty((rows,)) if want_rstd else None
+    lib.call("xsmi_rms_norm_fwd", x.read_ptr, residual.read_ptr if residual is not None else None, gamma.read_ptr,
+             s.ptr if residual is not None else None, y.ptr, rstd.ptr if want_rstd else None, rows, cols, eps)
+    return y, s, rstd
+
+
+def rms_norm_int8(x, gamma, eps, residual=None):
+    """(q, scale, s): the same rows as int8 numbers and a float32 scale each."""
+    rows, cols = _rms_operands(x, gamma, residual)
+    if cols == 0:
+        raise ValueError("rms_norm: rows without elements")
+    s = empty(x.shape) if residual is not None else x
+    q, scale = empty(x.shape, np.int8), empty(x.shape[:-1])
+    lib.call("xsmi_rms_norm_int8", x.read_ptr, residual.read_ptr if residual is not None else None, gamma.read_ptr,
+             s.ptr if residual is not None else None, q.ptr, scale.ptr, rows, cols, eps)
+    return q, scale, s
+
+
+def rms_norm_bwd(dy, s, rstd, gamma, ds=None, dx1=None, dx2=None, dgamma=None):
+    """Adds the gradient of the rows (and ``ds``, what reaches s another way) to dx1 and dx2, and that of the scales to dgamma;
+    each may be None, and one whose clear is pending is overwritten.  dx1 may be ds itself (which then is not added twice)."""
+    rows, cols = _rms_operands(s, gamma, None)
+    for a in (dy, ds, dx1, dx2):
+        if a is not None and (a.size != s.size or a.dtype != np.float32):
+            raise ValueError("rms_norm_bwd: operand of shape %s for rows of %s" % (a.shape, s.shape))
+    if rstd.size != rows or (dgamma is not None and (dgamma.size != cols or dgamma.dtype != np.float32)):
+        raise ValueError("rms_norm_bwd: operands do not match %s" % (s.shape,))
+    if ds is not None and ds.is_fresh():
+        ds = None
+    if ds is not None and ds is dx1:
+        ds = None
+    betas = [0.0 if a is None or a.take_fresh() else 1.0 for a in (dx1, dx2, dgamma)]
+    ws, ws_bytes = None, 0
+    if dgamma is not None and rows:
+        ws, ws_bytes = _ws.get(lib.raw("xsmi_rms_norm_workspace_bytes")(rows, cols))
+    p = [a.ptr if a is not None else None for a in (dx1, dx2, dgamma)]
+    lib.call("xsmi_rms_norm_bwd", dy.read_ptr, s.read_ptr, rstd.read_ptr, gamma.read_ptr, ds.read_ptr if ds is not None else None, p[0], betas[0],
+             p[1], betas[1], p[2], betas[2], rows, cols, ws, ws_bytes)
+
+
 # ---- AdamW -----------------------------------------------------------------------------------------------------
 def adamw_step(launch, moments, opt):
     """One step of ``optim.AdamW`` over the tensors of ``launch`` (its tables of addresses, which belong to arrays that it

@@ -1,0 +1,479 @@
+// Root-mean-square normalisation of rows, with the residual's addition in front of it, forward and backward, and with an
+// output in 8 bits.
+//
+//   s = x + residual        r = 1 / sqrt(mean_j s_j^2 + eps)        y_j = gamma_j s_j r
+//   backward, with a_j = gamma_j dy_j and xhat_j = s_j r:
+//     ds_j += r (a_j - xhat_j mean_i(a_i xhat_i))                   dgamma_j = sum_rows dy_j xhat_j
+//
+// All of it is bound by memory: a row is read once, kept in registers while its sum is formed, and written once.
+#include "xsmi_internal.h"
+#include <math.h>
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef f4 f4u __attribute__((aligned(4)));              // rows of an odd length start at any element
+
+// The sum over the T threads that share a row, in every one of them; T is a power of two, at least one wave's share of a row.
+template <int T, typename V>
+__device__ __forceinline__ V row_sum(V v, V *sm) {
+#pragma unroll
+    for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    if (T > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const int first = threadIdx.x / T * (T / 64);
+        v = sm[first];
+#pragma unroll
+        for (int w = 1; w < T / 64; ++w) v += sm[first + w];
+    }
+    return v;
+}
+
+template <int T>
+__device__ __forceinline__ double row_max(double v, double *sm) {
+#pragma unroll
+    for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
+    if (T > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const int first = threadIdx.x / T * (T / 64);
+        v = sm[first];
+#pragma unroll
+        for (int w = 1; w < T / 64; ++w) v = fmax(v, sm[first + w]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ f4 load4(const float *p, int j, int cols) {
+    if (j + 4 <= cols) return *reinterpret_cast<const f4u *>(p + j);
+    f4 r = {0.f, 0.f, 0.f, 0.f};
+    if (j < cols) r.x = p[j];
+    if (j + 1 < cols) r.y = p[j + 1];
+    if (j + 2 < cols) r.z = p[j + 2];
+    return r;
+}
+
+__device__ __forceinline__ void store4(float *p, int j, int cols, f4 v) {
+    if (j + 4 <= cols) {
+        *reinterpret_cast<f4u *>(p + j) = v;
+        return;
+    }
+    if (j < cols) p[j] = v.x;
+    if (j + 1 < cols) p[j + 1] = v.y;
+    if (j + 2 < cols) p[j + 2] = v.z;
+}
+
+struct Forward {
+    const float *x, *residual, *gamma;
+    float *sum, *y, *rstd;
+    int8_t *q;
+    float *scale;
+    uint64_t rows;
+    int cols;
+    float eps;
+};
+
+// T threads a row, NT threads a workgroup, V vectors of four a thread: rows of up to 4 T V elements stay in registers.
+template <int T, int NT, int V>
+__global__ void __launch_bounds__(NT) rms_fwd_kernel(Forward a) {
+    __shared__ float sm[NT / 64];
+    const uint64_t row = (uint64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
+    const int t = threadIdx.x % T, cols = a.cols;
+    const bool live = row < a.rows;
+    const uint64_t at = row * (uint64_t)cols;
+    f4 s[V];
+    float sq = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int j = 4 * (v * T + t);
+        s[v] = f4{0.f, 0.f, 0.f, 0.f};
+        if (live && j < cols) {
+            s[v] = load4(a.x + at, j, cols);
+            if (a.residual) s[v] += load4(a.residual + at, j, cols);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sq += s[v][e] * s[v][e];
+    sq = row_sum<T>(sq, sm);
+    const float r = 1.f / sqrtf(sq / (float)cols + a.eps);
+    if (!live) return;
+    if (t == 0 && a.rstd) a.rstd[row] = r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int j = 4 * (v * T + t);
+        if (j < cols) {
+            if (a.sum) store4(a.sum + at, j, cols, s[v]);
+            store4(a.y + at, j, cols, s[v] * r * load4(a.gamma, j, cols));
+        }
+    }
+}
+
+// Longer rows: a workgroup reads its row twice.
+template <int NT>
+__global__ void __launch_bounds__(NT) rms_fwd_long_kernel(Forward a) {
+    __shared__ float sm[NT / 64];
+    const uint64_t row = blockIdx.x, at = row * (uint64_t)a.cols;
+    const int cols = a.cols;
+    float sq = 0.f;
+    for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
+        f4 s = load4(a.x + at, j, cols);
+        if (a.residual) {
+            s += load4(a.residual + at, j, cols);
+            store4(a.sum + at, j, cols, s);
+        }
+        sq += (s.x * s.x + s.y * s.y) + (s.z * s.z + s.w * s.w);
+    }
+    sq = row_sum<NT>(sq, sm);
+    const float r = 1.f / sqrtf(sq / (float)cols + a.eps);
+    if (threadIdx.x == 0 && a.rstd) a.rstd[row] = r;
+    const float *s = a.residual ? a.sum + at : a.x + at;     // a thread reads what it has written itself
+    for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) store4(a.y + at, j, cols, load4(s, j, cols) * r * load4(a.gamma, j, cols));
+}
+
+// Four numbers of 8 bits, to the nearest, ties to even.
+__device__ __forceinline__ void store_q(int8_t *p, int j, int cols, const double *y, double inverse) {
+    int q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = (int)rint(y[e] * inverse);
+    if (j + 4 <= cols && ((uintptr_t)(p + j) & 3) == 0) {
+        *reinterpret_cast<uint32_t *>(p + j) = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)q[3] << 24;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < cols) p[j + e] = (int8_t)q[e];
+}
+
+// The output in 8 bits: q_j = round(127 y_j / max |y|), scale = max |y| / 127.  In 64 bits, which run at the rate of 32 here and
+// are not what bounds this: a number next to a border falls on the side that the exact value is on, whatever the order
+// of the sums.
+template <int T, int NT, int V>
+__global__ void __launch_bounds__(NT) rms_fwd_int8_kernel(Forward a) {
+    __shared__ double sm[NT / 64];
+    const uint64_t row = (uint64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
+    const int t = threadIdx.x % T, cols = a.cols;
+    const bool live = row < a.rows;
+    const uint64_t at = row * (uint64_t)cols;
+    f4 s[V];
+    double sq = 0.0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int j = 4 * (v * T + t);
+        s[v] = f4{0.f, 0.f, 0.f, 0.f};
+        if (live && j < cols) {
+            s[v] = load4(a.x + at, j, cols);
+            if (a.residual) {
+                s[v] += load4(a.residual + at, j, cols);
+                store4(a.sum + at, j, cols, s[v]);
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sq += (double)s[v][e] * (double)s[v][e];
+    sq = row_sum<T>(sq, sm);
+    const double r = 1.0 / sqrt(sq / (double)cols + (double)a.eps);
+    double most = 0.0;
+    bool nan = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int j = 4 * (v * T + t);
+        if (live && j < cols) {
+            const f4 g = load4(a.gamma, j, cols);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double y = (double)s[v][e] * r * (double)g[e];
+                nan |= y != y;
+                most = fmax(most, fabs(y));
+            }
+        }
+    }
+    most = row_max<T>(nan ? INFINITY : most, sm);
+    if (!live) return;
+    // A row of zeros has the numbers 0 and the scale 0; one with a NaN or an infinity the numbers 0 and the scale NaN.
+    const bool bad = !(most < INFINITY);
+    const double inverse = bad || most == 0.0 ? 0.0 : 127.0 / most;
+    if (t == 0) a.scale[row] = bad ? NAN : (float)(most / 127.0);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int j = 4 * (v * T + t);
+        if (j < cols) {
+            const f4 g = load4(a.gamma, j, cols);
+            double y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = bad ? 0.0 : (double)s[v][e] * r * (double)g[e];
+            store_q(a.q + at, j, cols, y, inverse);
+        }
+    }
+}
+
+template <int NT>
+__global__ void __launch_bounds__(NT) rms_fwd_int8_long_kernel(Forward a) {
+    __shared__ double sm[NT / 64];
+    const uint64_t row = blockIdx.x, at = row * (uint64_t)a.cols;
+    const int cols = a.cols;
+    double sq = 0.0;
+    for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
+        f4 s = load4(a.x + at, j, cols);
+        if (a.residual) {
+            s += load4(a.residual + at, j, cols);
+            store4(a.sum + at, j, cols, s);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sq += (double)s[e] * (double)s[e];
+    }
+    sq = row_sum<NT>(sq, sm);
+    const double r = 1.0 / sqrt(sq / (double)cols + (double)a.eps);
+    const float *from = a.residual ? a.sum + at : a.x + at;
+    double most = 0.0;
+    bool nan = false;
+    for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
+        const f4 s = load4(from, j, cols), g = load4(a.gamma, j, cols);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double y = (double)s[e] * r * (double)g[e];
+            nan |= y != y;
+            most = fmax(most, fabs(y));
+        }
+    }
+    most = row_max<NT>(nan ? INFINITY : most, sm);
+    const bool bad = !(most < INFINITY);
+    const double inverse = bad || most == 0.0 ? 0.0 : 127.0 / most;
+    if (threadIdx.x == 0) a.scale[row] = bad ? NAN : (float)(most / 127.0);
+    for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
+        const f4 s = load4(from, j, cols), g = load4(a.gamma, j, cols);
+        double y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = bad ? 0.0 : (double)s[e] * r * (double)g[e];
+        store_q(a.q + at, j, cols, y, inverse);
+    }
+}
+
+struct Backward {
+    const float *dy, *s, *rstd, *gamma, *ds;
+    float *dx1, *dx2, *part;
+    int acc1, acc2;
+    uint64_t rows;
+    int cols;
+};
+
+// T threads a row; a workgroup takes every (NT / T gridDim)-th lot of rows, and adds the terms of dgamma of the columns
+// that a thread owns in its registers; they go to part[group of rows] at the end.
+template <int T, int NT, int V>
+__global__ void __launch_bounds__(NT) rms_bwd_kernel(Backward a) {
+    __shared__ float sm[NT / 64];
+    const int t = threadIdx.x % T, cols = a.cols;
+    const float inv = 1.f / (float)cols;
+    f4 dg[V], gm[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int j = 4 * (v * T + t);
+        dg[v] = f4{0.f, 0.f, 0.f, 0.f};
+        gm[v] = j < cols ? load4(a.gamma, j, cols) : dg[v];
+    }
+    for (uint64_t first = (uint64_t)blockIdx.x * (NT / T); first < a.rows; first += (uint64_t)gridDim.x * (NT / T)) {
+        const uint64_t row = first + threadIdx.x / T, at = row * (uint64_t)cols;
+        const bool live = row < a.rows;
+        f4 s[V], d[V];
+        float c = 0.f;
+        const float r = live ? a.rstd[row] : 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int j = 4 * (v * T + t);
+            s[v] = d[v] = f4{0.f, 0.f, 0.f, 0.f};
+            if (live && j < cols) {
+                s[v] = load4(a.s + at, j, cols);
+                d[v] = load4(a.dy + at, j, cols);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            s[v] *= r;
+            dg[v] += d[v] * s[v];
+            d[v] *= gm[v];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c += d[v][e] * s[v][e];
+        }
+        c = row_sum<T>(c, sm) * inv;
+        if (live && a.dx1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int j = 4 * (v * T + t);
+                if (j < cols) {
+                    f4 g = (d[v] - s[v] * c) * r;
+                    if (a.ds) g += load4(a.ds + at, j, cols);
+                    f4 o = g;
+                    if (a.acc1) o += load4(a.dx1 + at, j, cols);
+                    store4(a.dx1 + at, j, cols, o);
+                    if (a.dx2) {
+                        o = g;
+                        if (a.acc2) o += load4(a.dx2 + at, j, cols);
+                        store4(a.dx2 + at, j, cols, o);
+                    }
+                }
+            }
+        }
+    }
+    if (a.part) {
+        float *part = a.part + ((uint64_t)blockIdx.x * (NT / T) + threadIdx.x / T) * (uint64_t)cols;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int j = 4 * (v * T + t);
+            if (j < cols) store4(part, j, cols, dg[v]);
+        }
+    }
+}
+
+// Longer rows, read twice; the terms of dgamma are added in memory, in this workgroup's own row of part.
+template <int NT>
+__global__ void __launch_bounds__(NT) rms_bwd_long_kernel(Backward a) {
+    __shared__ float sm[NT / 64];
+    const int cols = a.cols;
+    float *part = a.part ? a.part + (uint64_t)blockIdx.x * cols : nullptr;
+    for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const uint64_t at = row * (uint64_t)cols;
+        const float r = a.rstd[row];
+        float c = 0.f;
+        for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
+            const f4 s = load4(a.s + at, j, cols) * r, d = load4(a.dy + at, j, cols), x = d * s;
+            if (part) store4(part, j, cols, row == blockIdx.x ? x : load4(part, j, cols) + x);
+            const f4 w = x * load4(a.gamma, j, cols);
+            c += (w.x + w.y) + (w.z + w.w);
+        }
+        c = row_sum<NT>(c, sm) / (float)cols;
+        if (a.dx1)
+            for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
+                const f4 s = load4(a.s + at, j, cols) * r;
+                f4 g = (load4(a.dy + at, j, cols) * load4(a.gamma, j, cols) - s * c) * r;
+                if (a.ds) g += load4(a.ds + at, j, cols);
+                store4(a.dx1 + at, j, cols, a.acc1 ? g + load4(a.dx1 + at, j, cols) : g);
+                if (a.dx2) store4(a.dx2 + at, j, cols, a.acc2 ? g + load4(a.dx2 + at, j, cols) : g);
+            }
+    }
+}
+
+// dgamma[j] = (accumulate ? dgamma[j] : 0) + sum over the rows of part: 64 columns and 16 stretches of rows a workgroup.
+__global__ void __launch_bounds__(1024) rms_dgamma_kernel(const float *__restrict__ part, int rows, int cols, float *dgamma, int accumulate) {
+    __shared__ float sm[16][64];
+    const int j = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    float s = 0.f;
+    if (j < cols)
+        for (int i = w; i < rows; i += 16) s += part[(uint64_t)i * cols + j];
+    sm[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w == 0 && j < cols) {
+        float r = 0.f;
+        for (int i = 0; i < 16; ++i) r += sm[i][threadIdx.x];
+        dgamma[j] = accumulate ? dgamma[j] + r : r;
+    }
+}
+
+constexpr uint64_t MAX_ROWS = 1ull << 31;
+
+// Workgroups of the backward, and the rows of part that they write.
+struct BackwardPlan {
+    int threads_a_row, threads, groups, parts;
+};
+BackwardPlan backward_plan(uint64_t rows, int cols) {
+    BackwardPlan p;
+    const int need = (cols + 3) / 4;
+    p.threads_a_row = need <= 16 ? 16 : need <= 64 ? 64 : need <= 1024 ? 256 : 1024;
+    p.threads = p.threads_a_row == 1024 ? 1024 : 256;
+    const uint64_t lots = (rows + p.threads / p.threads_a_row - 1) / (p.threads / p.threads_a_row);
+    const uint64_t most = p.threads == 1024 ? 256 : 1024;
+    p.groups = (int)(lots < most ? lots : most);
+    p.parts = p.groups * (p.threads / p.threads_a_row);
+    return p;
+}
+
+int check(const char *who, size_t rows, int cols, float eps) {
+    XSMI_CHECK_ARG(cols >= 1 && cols <= (1 << 30), "%s: %d columns", who, cols);
+    XSMI_CHECK_ARG(rows < MAX_ROWS, "%s: %zu rows", who, rows);
+    XSMI_CHECK_ARG(eps >= 0, "%s: epsilon %g", who, (double)eps);
+    return XSMI_OK;
+}
+
+#define LAUNCH(kernel, grid, threads, args) hipLaunchKernelGGL(kernel, dim3((uint32_t)(grid)), dim3(threads), 0, xsmi::stream(), args)
+
+}  // namespace
+
+extern "C" {
+
+int xsmi_rms_norm_fwd(const float *x, const float *residual, const float *gamma, float *sum, float *y, float *rstd, size_t rows, int cols,
+                      float eps) {
+    XSMI_REQUIRE_INIT();
+    if (int rc = check("xsmi_rms_norm_fwd", rows, cols, eps)) return rc;
+    if (rows == 0) return XSMI_OK;
+    XSMI_CHECK_ARG(x && gamma && y && (residual == nullptr) == (sum == nullptr), "xsmi_rms_norm_fwd: null pointer (a residual comes with a sum)");
+    const Forward a = {x, residual, gamma, sum, y, rstd, nullptr, nullptr, rows, cols, eps};
+    const int need = (cols + 3) / 4;
+    if (need <= 16) LAUNCH((rms_fwd_kernel<16, 256, 1>), (rows + 15) / 16, 256, a);
+    else if (need <= 64) LAUNCH((rms_fwd_kernel<64, 256, 1>), (rows + 3) / 4, 256, a);
+    else if (need <= 256) LAUNCH((rms_fwd_kernel<256, 256, 1>), rows, 256, a);
+    else if (need <= 1024) LAUNCH((rms_fwd_kernel<256, 256, 4>), rows, 256, a);
+    else if (need <= 4096) LAUNCH((rms_fwd_kernel<1024, 1024, 4>), rows, 1024, a);
+    else LAUNCH((rms_fwd_long_kernel<1024>), rows, 1024, a);
+    XSMI_LAUNCH_CHECK("rms_fwd_kernel");
+    return XSMI_OK;
+}
+
+int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma, float *sum, int8_t *q, float *scale, size_t rows, int cols,
+                       float eps) {
+    XSMI_REQUIRE_INIT();
+    if (int rc = check("xsmi_rms_norm_int8", rows, cols, eps)) return rc;
+    if (rows == 0) return XSMI_OK;
+    XSMI_CHECK_ARG(x && gamma && q && scale && (residual == nullptr) == (sum == nullptr), "xsmi_rms_norm_int8: null pointer (a residual comes with a sum)");
+    const Forward a = {x, residual, gamma, sum, nullptr, nullptr, q, scale, rows, cols, eps};
+    const int need = (cols + 3) / 4;
+    if (need <= 16) LAUNCH((rms_fwd_int8_kernel<16, 256, 1>), (rows + 15) / 16, 256, a);
+    else if (need <= 64) LAUNCH((rms_fwd_int8_kernel<64, 256, 1>), (rows + 3) / 4, 256, a);
+    else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1>), rows, 256, a);
+    else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<256, 256, 4>), rows, 256, a);
+    else if (need <= 4096) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 4>), rows, 1024, a);
+    else LAUNCH((rms_fwd_int8_long_kernel<1024>), rows, 1024, a);
+    XSMI_LAUNCH_CHECK("rms_fwd_int8_kernel");
+    return XSMI_OK;
+}
+
+size_t xsmi_rms_norm_workspace_bytes(size_t rows, int cols) {
+    if (rows == 0 || rows >= MAX_ROWS || cols < 1 || cols > (1 << 30)) return 0;
+    return (size_t)backward_plan(rows, cols).parts * (size_t)cols * sizeof(float);
+}
+
+int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const float *gamma, const float *ds, float *dx1, float beta1,
+                      float *dx2, float beta2, float *dgamma, float beta_gamma, size_t rows, int cols, void *ws, size_t ws_bytes) {
+    XSMI_REQUIRE_INIT();
+    if (int rc = check("xsmi_rms_norm_bwd", rows, cols, 0.f)) return rc;
+    XSMI_CHECK_ARG((beta1 == 0.f || beta1 == 1.f) && (beta2 == 0.f || beta2 == 1.f) && (beta_gamma == 0.f || beta_gamma == 1.f),
+                   "xsmi_rms_norm_bwd: beta is 0 or 1");
+    XSMI_CHECK_ARG(!dx2 || (dx1 && dx1 != dx2), "xsmi_rms_norm_bwd: a second gradient comes beside the first, in memory of its own");
+    if (rows == 0) return dgamma && beta_gamma == 0.f ? xsmi_fill(dgamma, 0.f, (size_t)cols) : XSMI_OK;
+    XSMI_CHECK_ARG(dy && s && rstd && gamma, "xsmi_rms_norm_bwd: null pointer");
+    const size_t want = dgamma ? xsmi_rms_norm_workspace_bytes(rows, cols) : 0;
+    XSMI_CHECK_ARG(ws_bytes >= want && (ws || !want) && ((uintptr_t)ws & 15) == 0, "xsmi_rms_norm_bwd: workspace of %zu bytes, needs %zu", ws_bytes, want);
+    if (!dx1 && !dgamma) return XSMI_OK;
+    const BackwardPlan p = backward_plan(rows, cols);
+    const Backward a = {dy, s, rstd, gamma, ds, dx1, dx2, dgamma ? (float *)ws : nullptr, beta1 != 0.f, beta2 != 0.f, rows, cols};
+    const int need = (cols + 3) / 4;
+    if (need <= 16) LAUNCH((rms_bwd_kernel<16, 256, 1>), p.groups, 256, a);
+    else if (need <= 64) LAUNCH((rms_bwd_kernel<64, 256, 1>), p.groups, 256, a);
+    else if (need <= 256) LAUNCH((rms_bwd_kernel<256, 256, 1>), p.groups, 256, a);
+    else if (need <= 1024) LAUNCH((rms_bwd_kernel<256, 256, 4>), p.groups, 256, a);
+    else if (need <= 4096) LAUNCH((rms_bwd_kernel<1024, 1024, 4>), p.groups, 1024, a);
+    else LAUNCH((rms_bwd_long_kernel<1024>), p.groups, 1024, a);
+    XSMI_LAUNCH_CHECK("rms_bwd_kernel");
+    if (dgamma) {
+        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((cols + 63) / 64), dim3(1024), 0, xsmi::stream(), (const float *)ws, p.parts, cols, dgamma,
+                           beta_gamma != 0.f);
+        XSMI_LAUNCH_CHECK("rms_dgamma_kernel");
+    }
+    return XSMI_OK;
+}
+
+}  // extern "C"

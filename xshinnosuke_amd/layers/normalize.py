@@ -1,4 +1,4 @@
-"""BatchNormalization (counterpart of xs/layers/normalize.py:22-56)."""
+"""BatchNormalization (counterpart of xs/layers/normalize.py:22-56) and RMSNormalization (this package's own)."""
 from ..core import state as GLOBAL
 from .base import Layer, F, Parameter
 from ..nn.initializers import get_initializer
@@ -32,3 +32,26 @@ class BatchNormalization(Layer):
         self._data = F.batch_norm(x, gamma, beta, self.moving_mean, self.moving_variance, self.axis, GLOBAL.TRAINING,
                                   self.epsilon, self.momentum, self._data, 'relu' if fuse_relu else None)
         return self._data
+
+
+class RMSNormalization(Layer):
+    """``gamma * s / sqrt(mean(s^2) + epsilon)`` over the last axis, ``s = x`` or, called as ``layer(x, residual)`` on
+    tensors, ``x + residual``: the result is then ``(y, s)``."""
+
+    def __init__(self, epsilon=1e-6, gamma_initializer='ones', **kwargs):
+        self.epsilon = epsilon
+        self.gamma_initializer = get_initializer(gamma_initializer)
+        super().__init__(**kwargs)
+
+    def init_params(self, input_shape=None, *args):
+        if input_shape is not None:
+            self._input_shape = tuple(input_shape)
+        self._parameters.append(Parameter(self.gamma_initializer(self._input_shape[-1], requires_grad=True)))
+
+    def call(self, x, residual=None, *args, **kwargs):
+        out = self._data
+        if out is not None and out.eval is not None and tuple(out.shape) != tuple(x.shape):
+            out = None
+        y = F.rms_norm(x, self._parameters[0], residual, self.epsilon, out)
+        self._data = y if residual is None else y[0]
+        return y

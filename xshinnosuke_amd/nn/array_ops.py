@@ -196,6 +196,24 @@ def batch_norm_backward(dy, xhat, sqrtvar, gamma):
     return dx, dgamma, dbeta
 
 
+def rms_norm(x, gamma, eps, residual=None, out=None):
+    """(y, s, rstd) over rows of the last axis; s = x + residual, or x itself.  A device ``out`` of the right size
+    receives y directly."""
+    if is_device(x):
+        y = out if (out is not None and is_device(out) and out.size == x.size) else None
+        return K.rms_norm_fwd(x, same_place(x, gamma).reshape(-1), eps, None if residual is None else same_place(x, residual), y=y)
+    s = x if residual is None else x + np.asarray(same_place(x, residual))
+    rstd = 1 / np.sqrt(np.mean(s * s, axis=-1, keepdims=True) + eps)
+    return (s * rstd * np.asarray(same_place(x, gamma)).reshape(-1)).astype(x.dtype, copy=False), s, rstd
+
+
+def rms_norm_backward(dy, s, rstd, gamma):
+    """Host arrays: the gradient of s and that of gamma."""
+    xhat = s * rstd
+    a = dy * gamma.reshape(-1)
+    return rstd * (a - xhat * np.mean(a * xhat, axis=-1, keepdims=True)), (dy * xhat).reshape(-1, s.shape[-1]).sum(axis=0)
+
+
 def avg_pool_blocks(x, k, stride=None):
     """Mean over k x k windows at the given stride (default k: non-overlapping blocks), no padding: the im2col
     mode of the reference's avg_pool2d, float64 sum and one rounding."""

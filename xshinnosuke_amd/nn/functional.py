@@ -512,6 +512,64 @@ def batch_norm(inputs, gamma, beta, moving_mean, moving_variance, axis=1, traini
     return out
 
 
+def rms_norm(inputs, gamma, residual=None, epsilon=1e-6, out=None):
+    """``gamma * s / sqrt(mean(s^2) + epsilon)`` over the last axis, with ``s = inputs + residual``, or ``inputs`` without
+    one (this package's extension).  ``residual`` has the shape of ``inputs``; with it the result is ``(y, s)``, s being what the next
+    residual addition takes.  On the device the addition and the normalisation are one pass, and so are their
+    backwards.  The backward reads s (``inputs`` without a residual) again: it must not be overwritten in place before."""
+    _mark_input(inputs)
+    if residual is not None and tuple(residual.shape) != tuple(inputs.shape):
+        raise ValueError('rms_norm: residual %s and input %s differ' % (residual.shape, inputs.shape))
+    if gamma.eval.size != inputs.shape[-1]:
+        raise ValueError('rms_norm: %d scales for rows of shape %s' % (gamma.eval.size, inputs.shape))
+    if not epsilon >= 0:
+        raise ValueError('rms_norm: epsilon must not be negative')
+    dst = None if out is None else out.eval
+    y, s, rstd = A.rms_norm(inputs.eval, gamma.eval, epsilon, None if residual is None else residual.eval, dst)
+    if out is None:
+        out = Tensor(y)
+    elif y is not dst:
+        out.eval = y
+    src = inputs
+    if residual is not None:
+        src = Tensor(s)
+        src.requires_grad = bool(inputs.requires_grad or residual.requires_grad)
+        _wire(src, inputs, residual)
+        if GLOBAL.COMPUTE_GRAD and src.requires_grad:
+            src.grad_fn = ResidualSumBackward
+            initialize_ops_grad(inputs, residual)
+    out.requires_grad = bool(src.requires_grad or gamma.requires_grad)
+    _wire(out, src, gamma)
+    if GLOBAL.COMPUTE_GRAD and out.requires_grad:
+        out.cache['rstd'] = rstd
+        out.grad_fn = RMSNormBackward
+        initialize_ops_grad(src, gamma)
+    return out if residual is None else (out, src)
+
+
+def rms_norm_8bit(inputs, gamma, residual=None, epsilon=1e-6):
+    """``rms_norm`` with its output in 8 bits: ``(q, scale)``, or ``(q, scale, s)`` with a residual.  Each row of q is int8
+    numbers, ``round(127 y / max |y|)``, that times its ``scale``, ``max |y| / 127``, stand for y: what ``dense_4bit`` takes.  Host
+    tensors are staged through the device.  Forward only."""
+    _mark_input(inputs)
+    _forward_only('rms_norm_8bit', inputs, gamma, residual)
+    if residual is not None and tuple(residual.shape) != tuple(inputs.shape):
+        raise ValueError('rms_norm_8bit: residual %s and input %s differ' % (residual.shape, inputs.shape))
+    if not epsilon >= 0:
+        raise ValueError('rms_norm_8bit: epsilon must not be negative')
+    x = inputs.eval
+    q, scale, s = K.rms_norm_int8(_f32_device(x), _f32_device(gamma.eval).reshape(-1), epsilon,
+                                  None if residual is None else _f32_device(residual.eval))
+    if not is_device(x):
+        q, scale, s = q.numpy(), scale.numpy().astype(x.dtype, copy=False), s.numpy().astype(x.dtype, copy=False)
+    return (Tensor(q), Tensor(scale)) if residual is None else (Tensor(q), Tensor(scale), Tensor(s))
+
+
+def _forward_only(what, *tensors):
+    if GLOBAL.COMPUTE_GRAD and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError('%s has no backward: call it under no_grad()' % what)
+
+
 def cross_entropy(x1, x2, reduction='mean', out=None):
     """Softmax + negative log-likelihood on integer labels (reference xs/nn/functional.py:984-1010)."""
     _mark_input(x1)

@@ -318,6 +318,56 @@ def BatchNormBackward(outputs):
         _accumulate(inputs, dx)
 
 
+def _add_rms_norm_grad(src, gamma, dy, rstd):
+    """The gradients of rms_norm's rows and scales, added to theirs."""
+    s = src.eval
+    if not is_device(s):
+        dx, dgamma = A.rms_norm_backward(np.asarray(A.same_place(s, dy)), s, rstd, np.asarray(A.same_place(s, gamma.eval)))
+        if src.requires_grad:
+            _accumulate(src, dx)
+        if gamma.requires_grad:
+            _accumulate(gamma, dgamma)
+        return
+    to = [t.grad.eval if t.requires_grad else None for t in (src, gamma)]
+    mine = [a if a is None or is_device(a) else dev.zeros(a.shape, lazy=True) for a in to]
+    K.rms_norm_bwd(A.same_place(s, dy), s, rstd, A.same_place(s, gamma.eval).reshape(-1), dx1=mine[0], dgamma=mine[1])
+    for t, a, b in zip((src, gamma), to, mine):
+        if a is not b:
+            _accumulate(t, b)
+
+
+def RMSNormBackward(outputs):
+    src, gamma = outputs.in_bounds
+    dy, rstd = outputs.grad.eval, outputs.cache['rstd']
+    if src.grad_fn is ResidualSumBackward and is_device(src.eval) and is_device(dy) and not src.retain_grad():
+        # s = x + residual is next but one at the latest: its own gradient is whole by then, and both go to the addends in one pass
+        src.cache['normed'] = (gamma, dy, rstd)
+    else:
+        _add_rms_norm_grad(src, gamma, dy, rstd)
+
+
+def ResidualSumBackward(outputs):
+    """Of s = inputs + residual in rms_norm, with the normalisation's own gradient where that has been left to it."""
+    waiting = outputs.cache.pop('normed', None)
+    if waiting is None:
+        AddBackward(outputs)
+        return
+    gamma, dy, rstd = waiting
+    s, ds = outputs.eval, outputs.grad.eval
+    to = [t for t in outputs.in_bounds if t.requires_grad]
+    grads = [t.grad.eval for t in to]
+    scale = gamma.grad.eval if gamma.requires_grad else None
+    fits = [is_device(a) and a.dtype == np.float32 and a.size == s.size for a in grads] + [scale is None or is_device(scale)]
+    if len(grads) == 2 and fits[0] and fits[1]:
+        fits.append(abs(grads[0].address() - grads[1].address()) >= s.nbytes)
+    if all(fits):
+        K.rms_norm_bwd(dy, s, rstd, A.same_place(s, gamma.eval).reshape(-1), ds, grads[0], grads[1] if len(grads) == 2 else None, scale)
+        outputs._grad = None                         # it has never held the normalisation's part
+    else:                                            # both addends one tensor, or gradients on the host
+        _add_rms_norm_grad(outputs, gamma, dy, rstd)
+        AddBackward(outputs)
+
+
 def CrossEntropyLossBackward(outputs):
     """Reference xs/nn/grad_fn.py:604-620."""
     logits, labels = outputs.in_bounds

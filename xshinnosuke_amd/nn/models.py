@@ -345,7 +345,8 @@ class Module(_Base):
     def __call__(self, x, *args, **kwargs):
         out = self.forward(x)
         self._collect(x)
-        out.is_leaf = True
+        for t in out if isinstance(out, (tuple, list)) else (out,):      # a residual block returns (y, the stream)
+            t.is_leaf = True
         return out
 
     def _collect(self, x):
