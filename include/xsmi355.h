@@ -478,6 +478,28 @@ size_t xsmi_rms_norm_workspace_bytes(size_t rows, int cols);
 int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const float *gamma, const float *ds, float *dx1, float beta1,
                       float *dx2, float beta2, float *dgamma, float beta_gamma, size_t rows, int cols, void *ws, size_t ws_bytes);
 
+/* ---- dense layers with weights in 4 bits ------------------------------------------------------------------------
+ * A weight of input k and output n is c scale, c a whole number in -8 .. 7 and scale a float16 that `group` (32, 64 or 128)
+ * inputs of an output share.  K inputs are padded to a multiple of 128, N outputs to one of 16.  codes
+ * (xsmi_dense_4bit_code_bytes, aligned to 16 bytes) is [outputs / 16][inputs / 128][64][16] bytes: lane l of chunk c of tile t holds
+ * output 16 t + l % 16; the low four bits of its byte 4 j + b are input 128 c + 32 j + 8 (l / 16) + 2 b and the high four the input
+ * after it, in two's complement.  scales (xsmi_dense_4bit_scale_count float16 values, aligned to 8 bytes) is
+ * [inputs / group][outputs].  Codes and scales of the padding have to be there, finite; the codes of the inputs behind the last one zero.
+ * xsmi_quantize_4bit makes them from a dense layer's w (K, N): a group's value of largest magnitude becomes -8, whatever
+ * its sign, the others go to the nearest number; values of 5e5 and more overflow the scale.  xsmi_dequantize_4bit
+ * writes the values (K, N) that they stand for.
+ * xsmi_dense_4bit: y (M, N) = x (M, K) . weights (+ bias[N] or NULL).  x_scale NULL: x is float32; else x is int8 rows with
+ * a float32 scale each, as xsmi_rms_norm_int8 writes them.  The workspace (needed for more rows than one
+ * matrix instruction holds) is sized by the query, x_bits 32 or 8; M below 2^21.  The order of all sums depends on the
+ * sizes alone.  The reference's dense layer is xs/nn/functional.py:99-120. */
+size_t xsmi_dense_4bit_code_bytes(int K, int N);
+size_t xsmi_dense_4bit_scale_count(int K, int N, int group);
+size_t xsmi_dense_4bit_workspace_bytes(size_t M, int K, int N, int x_bits);
+int xsmi_quantize_4bit(const float *w, int K, int N, int group, uint8_t *codes, void *scales);
+int xsmi_dequantize_4bit(const uint8_t *codes, const void *scales, int K, int N, int group, float *w);
+int xsmi_dense_4bit(const void *x, const float *x_scale, const uint8_t *codes, const void *scales, const float *bias, float *y, size_t M, int K,
+                    int N, int group, void *ws, size_t ws_bytes);
+
 /* ---- optimizer: AdamW over many tensors ------------------------------------------------------------------------
  *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
  *   p' = p (1 - lr weight_decay) - lr m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps)

@@ -116,6 +116,12 @@ SIGNATURES = {
     "xsmi_rms_norm_int8": (_i, [_vp] * 6 + [_sz, _i, _f]),
     "xsmi_rms_norm_workspace_bytes": (_sz, [_sz, _i]),
     "xsmi_rms_norm_bwd": (_i, [_vp] * 6 + [_f, _vp, _f, _vp, _f, _sz, _i, _vp, _sz]),
+    "xsmi_dense_4bit_code_bytes": (_sz, [_i, _i]),
+    "xsmi_dense_4bit_scale_count": (_sz, [_i, _i, _i]),
+    "xsmi_dense_4bit_workspace_bytes": (_sz, [_sz, _i, _i, _i]),
+    "xsmi_quantize_4bit": (_i, [_vp, _i, _i, _i, _vp, _vp]),
+    "xsmi_dequantize_4bit": (_i, [_vp, _vp, _i, _i, _i, _vp]),
+    "xsmi_dense_4bit": (_i, [_vp] * 6 + [_sz, _i, _i, _i, _vp, _sz]),
     "xsmi_adamw_step": (_i, [_i] + [_vp] * 8 + [_sz, _i] + [_c.c_double] * 5 + [_c.c_uint32, _vp]),
     "xsmi_adamw_moments": (_i, [_vp] * 6 + [_sz]),
     "xsmi_graph_begin": (_i, []),
@@ -179,7 +185,8 @@ class _Lib:
 
 
 _QUERIES = frozenset(("xsmi_scratch_bytes", "xsmi_conv2d_workspace_bytes", "xsmi_conv2d_pass_workspace_bytes", "xsmi_bn_workspace_bytes",
-                      "xsmi_rms_norm_workspace_bytes", "xsmi_conv2d_bwd_pending", "xsmi_is_initialized", "xsmi_last_error"))
+                      "xsmi_rms_norm_workspace_bytes", "xsmi_dense_4bit_code_bytes", "xsmi_dense_4bit_scale_count",
+                      "xsmi_dense_4bit_workspace_bytes", "xsmi_conv2d_bwd_pending", "xsmi_is_initialized", "xsmi_last_error"))
 
 lib = _Lib()
 

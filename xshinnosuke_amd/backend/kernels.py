@@ -909,6 +909,59 @@ def rms_norm_bwd(dy, s, rstd, gamma, ds=None, dx1=None, dx2=None, dgamma=None):
              p[1], betas[1], p[2], betas[2], rows, cols, ws, ws_bytes)
 
 
+# ---- dense layers with weights in 4 bits -------------------------------------------------------------------------
+def dense_4bit_shapes(inputs, outputs, group):
+    """Shapes of the codes (uint8) and scales (float16) of a packed weight."""
+    count = lib.raw("xsmi_dense_4bit_scale_count")(inputs, outputs, group)
+    if not count:
+        raise ValueError("a 4-bit weight of %s inputs, %s outputs and groups of %s (expected 32, 64 or 128)" % (inputs, outputs, group))
+    cols = -(-outputs // 16) * 16
+    return (cols // 16, -(-inputs // 128), 64, 16), (count // cols, cols)
+
+
+def quantize_4bit(w, group):
+    """(codes, scales) of a dense layer's (inputs, outputs) weight."""
+    _f32(w, "w")
+    if len(w.shape) != 2:
+        raise ValueError("quantize_4bit: weight of shape %s" % (w.shape,))
+    codes, scales = dense_4bit_shapes(*w.shape, group)
+    codes, scales = empty(codes, np.uint8), empty(scales, np.float16)
+    lib.call("xsmi_quantize_4bit", w.read_ptr, w.shape[0], w.shape[1], group, codes.ptr, scales.ptr)
+    return codes, scales
+
+
+def dequantize_4bit(codes, scales, inputs, outputs, group):
+    w = empty((inputs, outputs))
+    lib.call("xsmi_dequantize_4bit", codes.read_ptr, scales.read_ptr, inputs, outputs, group, w.ptr)
+    return w
+
+
+def dense_4bit(x, codes, scales, inputs, outputs, group, bias=None, x_scale=None, out=None):
+    """x (rows, inputs) times the packed weight (+ bias over rows): float32 rows, or int8 rows with ``x_scale``."""
+    if x.dtype != (np.float32 if x_scale is None else np.int8):
+        raise ValueError("dense_4bit: rows of %s %s a scale" % (x.dtype, "without" if x_scale is None else "with"))
+    if not x.shape or x.shape[-1] != inputs:
+        raise ValueError("dense_4bit: rows of shape %s for %d inputs" % (x.shape, inputs))
+    rows = x.size // inputs
+    if x_scale is not None and (x_scale.size != rows or x_scale.dtype != np.float32):
+        raise ValueError("dense_4bit: %d scales for %d rows" % (x_scale.size, rows))
+    if bias is not None and (bias.size != outputs or bias.dtype != np.float32):
+        raise ValueError("dense_4bit: bias of %d elements for %d outputs" % (bias.size, outputs))
+    if out is None:
+        out = empty(x.shape[:-1] + (outputs,))
+    elif out.size != rows * outputs or out.dtype != np.float32:
+        raise ValueError("dense_4bit: output has shape %s, expected %s" % (out.shape, x.shape[:-1] + (outputs,)))
+    out.take_fresh()
+    key = ("dense4", rows, inputs, outputs, x_scale is None)
+    need = _NEED.get(key)
+    if need is None:
+        need = _NEED[key] = lib.raw("xsmi_dense_4bit_workspace_bytes")(rows, inputs, outputs, 32 if x_scale is None else 8)
+    ws, ws_bytes = _ws.get(need) if need else (None, 0)
+    lib.call("xsmi_dense_4bit", x.read_ptr, x_scale.read_ptr if x_scale is not None else None, codes.read_ptr, scales.read_ptr,
+             bias.read_ptr if bias is not None else None, out.ptr, rows, inputs, outputs, group, ws, ws_bytes)
+    return out
+
+
 # ---- AdamW -----------------------------------------------------------------------------------------------------
 def adamw_step(launch, moments, opt):
     """One step of ``optim.AdamW`` over the tensors of ``launch`` (its tables of addresses, which belong to arrays that it

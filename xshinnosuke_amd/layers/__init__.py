@@ -1,5 +1,5 @@
 from .base import Layer
-from .linear import Dense, Flatten
+from .linear import Dense, Dense4Bit, Flatten
 from .convolutional import Conv2D
 from .pooling import MaxPooling2D, AvgPooling2D
 from .normalize import BatchNormalization, RMSNormalization

@@ -1,9 +1,10 @@
-"""Dense and Flatten (counterpart of xs/layers/linear.py)."""
+"""Dense and Flatten (counterpart of xs/layers/linear.py), and Dense4Bit (this package's own)."""
 import math
 
-from .base import Layer, F, Parameter
-from .activators import FusedActivation
+from .base import Layer, F, Parameter, Tensor
+from .activators import Activation, FusedActivation
 from ..nn.initializers import get_initializer
+from ..nn.weight4 import Weight4Bit
 
 
 class Dense(FusedActivation, Layer):
@@ -46,6 +47,51 @@ class Dense(FusedActivation, Layer):
     def backward(self, gradients=None):
         self._act_backward()
         super().backward(gradients)
+
+
+class Dense4Bit(FusedActivation, Layer):
+    """A trained ``Dense`` with its weight in 4 bits, for inference: ``Dense4Bit.from_dense(layer, group)`` packs the weight and
+    takes over the bias and the activation.  It takes float32 rows, or, called as ``layer(q, scale=scale)``, the 8-bit rows of
+    ``rms_norm_8bit``.  It has no parameters to train and no backward."""
+
+    def __init__(self, weight, bias=None, activation=None, **kwargs):
+        if not isinstance(weight, Weight4Bit):
+            raise ValueError('Dense4Bit: weight must be a Weight4Bit')
+        self.weight, self.bias, self.out_features = weight, bias, weight.out_features
+        self._set_activation(activation, fuse_relu=False)
+        kwargs.setdefault('trainable', False)
+        kwargs.setdefault('input_shape', (weight.in_features,))
+        super().__init__(**kwargs)
+
+    @classmethod
+    def from_dense(cls, dense, group=128):
+        params = dense.parameters()
+        if not params:
+            raise ValueError('Dense4Bit: the layer has no weight yet')
+        bias = None
+        if dense.use_bias:
+            b = params[1].eval
+            bias = Tensor(F.to_device(b) if not F.is_device(b) else b.copy())
+        act = dense._act_layer
+        return cls(Weight4Bit.quantize(params[0], group), bias, act if isinstance(act, Activation) else act and type(act).__name__)
+
+    def compute_output_shape(self, input_shape=None):
+        self._shape = (self.out_features,)
+        return self._shape
+
+    def init_layer_out_tensor(self, x=None):
+        super().init_layer_out_tensor(x)
+        self._static_act_buffer()
+
+    def call(self, x, scale=None, *args, **kwargs):
+        out = self._data
+        if out is not None and (out.eval is None or tuple(out.shape) != tuple(x.shape[:-1]) + (self.out_features,)):
+            out = None
+        self._data = F.dense_4bit(x, self.weight, self.bias, scale, out)
+        return self._activate(self._data)
+
+    def backward(self, gradients=None):
+        raise NotImplementedError('Dense4Bit has no backward')
 
 
 class Flatten(Layer):

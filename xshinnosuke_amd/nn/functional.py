@@ -565,6 +565,34 @@ def rms_norm_8bit(inputs, gamma, residual=None, epsilon=1e-6):
     return (Tensor(q), Tensor(scale)) if residual is None else (Tensor(q), Tensor(scale), Tensor(s))
 
 
+def dense_4bit(inputs, weight, bias=None, scale=None, out=None):
+    """``inputs @ weight (+ bias)`` with a :class:`Weight4Bit` (this package's extension): float32 rows, or the int8 rows and
+    their ``scale`` that ``rms_norm_8bit`` gives.  The sums are those of float32 products, of 8-bit rows exact within a group.  Host
+    tensors are staged through the device.  Forward only."""
+    _mark_input(inputs)
+    _forward_only('dense_4bit', inputs, bias, scale)
+    x = inputs.eval
+    on_device = is_device(x)
+    if scale is not None and x.dtype != np.int8:
+        raise ValueError('dense_4bit: rows of %s with a scale, expected int8' % (x.dtype,))
+    if scale is None and np.dtype(x.dtype).kind != 'f':
+        raise ValueError('dense_4bit: rows of %s without a scale' % (x.dtype,))
+    x_dev = x if on_device else to_device(np.ascontiguousarray(x), np.float32 if scale is None else np.int8)
+    s_dev = None if scale is None else _f32_device(scale.eval)
+    b_dev = None if bias is None else _f32_device(bias.eval).reshape(-1)
+    dst = None if out is None else out.eval
+    y = weight.product(x_dev, b_dev, s_dev, dst if dst is not None and is_device(dst) else None)
+    if out is None:
+        kind = x.dtype if scale is None else scale.eval.dtype
+        out = Tensor(y if on_device else y.numpy().astype(kind, copy=False))
+    elif y is not dst:
+        out.eval = y
+    out.requires_grad = False
+    out.grad_fn = None
+    _wire(out, inputs)
+    return out
+
+
 def _forward_only(what, *tensors):
     if GLOBAL.COMPUTE_GRAD and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError('%s has no backward: call it under no_grad()' % what)
