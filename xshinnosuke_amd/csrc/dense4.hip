@@ -102,53 +102,57 @@ struct Dense {
 // ---- few rows ----------------------------------------------------------------------------------------------------
 // A workgroup of W waves has 16 outputs and splits their inputs over its waves, chunk by chunk; the rows go through LDS, in
 // windows of W PF chunks, and the waves' sums are added at the end.  A float32 row takes two of the 16 columns of a multiplication, one for
-// each part (rows 0 to 7 the first parts, 8 to 15 the second), an 8-bit row one.  Columns without a row repeat the last
-// one: a column's sums are its own.
+// each part (columns 0 to 7 the first parts, 8 to 15 the second), an 8-bit row one.  Columns without a row repeat the last
+// one: a column's sums are its own.  A window's loads are all under way before the first of them is needed: the rows' first, for
+// loads come back in order, then a wave's PF kilobytes of codes and their scales.
 template <int G, bool INT8, int W, int PF>
 __global__ void __launch_bounds__(W * 64) dense4_few_kernel(Dense a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ uint32_t most[W];
+    constexpr int GROUPS = 128 / G;                  // of a chunk
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, col = lane & 15;
     const int n0 = blockIdx.x * 16, M = a.M;
     const u4 *const codes = reinterpret_cast<const u4 *>(a.codes) + (uint64_t)blockIdx.x * a.chunks * 64 + lane;
     const _Float16 *const scales = a.scales + n0 + 4 * q;
     const int row = INT8 ? min(col, M - 1) : min(col & 7, M - 1);
+    // float32 rows: W / width waves for each of up to `width` rows; a thread has up to MINE octets of one
+    constexpr int MINE = 4;
+    static_assert(INT8 || W == 8, "128 PF octets a row: 4 of each thread for PF 8, 4, 2 and width 2, 4, 8");
+    const int width = M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8, waves = W / width, m = wave / waves, mine = (wave % waves) * 64 + lane;
     f4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int first = 0; first < a.chunks; first += W * PF) {
-        const int here = min(W * PF, a.chunks - first);
-        u4 w[PF];
-#pragma unroll
-        for (int i = 0; i < PF; ++i) {
-            const int c = wave + W * i;
-            if (c < here) w[i] = codes[(uint64_t)(first + c) * 64];
-        }
-        float back = 1.f;
-        f4 sum = {0.f, 0.f, 0.f, 0.f};
-        if (INT8) {
-            u2 *const to = reinterpret_cast<u2 *>(lds);
-            const int octets = here * 16;
-            for (int i = threadIdx.x; i < octets * M; i += W * 64) {
-                const int m = i / octets, o = i - m * octets;
-                to[o * M + m] = order_i8(load8(static_cast<const int8_t *>(a.x) + (uint64_t)m * a.K, first * 128 + o * 8, a.K));
-            }
-        } else {
-            // W / width waves for each of up to `width` rows; a thread has up to four octets of one
-            constexpr int MINE = 4;
-            static_assert(W == 8, "128 PF octets a row: 4 of each thread for PF 8, 4, 2 and width 2, 4, 8");
-            h8 *const to = reinterpret_cast<h8 *>(lds);
-            const int width = M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8, waves = W / width, m = wave / waves, mine = (wave % waves) * 64 + lane;
-            const int octets = here * 16;
-            float v[MINE][8];
-            uint32_t top = 0;
+        const int here = min(W * PF, a.chunks - first), octets = here * 16;
+        float v[MINE][8];
+        if (!INT8) {
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
                 const int o = mine + i * waves * 64;
-                if (m < M && o < octets) {
-                    load8(static_cast<const float *>(a.x) + (uint64_t)m * a.K, first * 128 + o * 8, a.K, v[i]);
+                if (m < M && o < octets) load8(static_cast<const float *>(a.x) + (uint64_t)m * a.K, first * 128 + o * 8, a.K, v[i]);
+            }
+        } else {
+            u2 *const to = reinterpret_cast<u2 *>(lds);
+            for (int r = 0; r < M; ++r)
+                for (int o = threadIdx.x; o < octets; o += W * 64)
+                    to[o * M + r] = order_i8(load8(static_cast<const int8_t *>(a.x) + (uint64_t)r * a.K, first * 128 + o * 8, a.K));
+        }
+        u4 w[PF];
+        h4 s[PF][GROUPS];
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int c = first + min(wave + W * i, here - 1);
+            w[i] = codes[(uint64_t)c * 64];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) s[i][g] = *reinterpret_cast<const h4 *>(scales + (uint64_t)(c * GROUPS + g) * a.cols);
+        }
+        float back = 1.f;
+        if (!INT8) {
+            h8 *const to = reinterpret_cast<h8 *>(lds);
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < MINE; ++i)
+                if (m < M && mine + i * waves * 64 < octets)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) top = max(top, size_bits(v[i][e]));
-                }
-            }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
             if (lane == 0) most[wave] = top;
@@ -174,13 +178,13 @@ __global__ void __launch_bounds__(W * 64) dense4_few_kernel(Dense a) {
             }
         }
         __syncthreads();
+        f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
             const int c = wave + W * i;
             if (c < here) {
 #pragma unroll
-                for (int g = 0; g < 128 / G; ++g) {
-                    const h4 s = *reinterpret_cast<const h4 *>(scales + (uint64_t)((first + c) * (128 / G) + g) * a.cols);
+                for (int g = 0; g < GROUPS; ++g) {
                     if (INT8) {
                         i4 d = {0, 0, 0, 0};
                         const u2 *const from = reinterpret_cast<const u2 *>(lds);
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(W * 64) dense4_few_kernel(Dense a) {
                             }
                         }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] += (float)s[e] * (float)d[e];
+                        for (int e = 0; e < 4; ++e) sum[e] += (float)s[i][g][e] * (float)d[e];
                     } else {
                         f4 d = {0.f, 0.f, 0.f, 0.f};
                         const h8 *const from = reinterpret_cast<const h8 *>(lds);
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(W * 64) dense4_few_kernel(Dense a) {
                         for (int j = g * (G / 32); j < (g + 1) * (G / 32); ++j)
                             d = __builtin_amdgcn_mfma_f32_16x16x32_f16(weights_f16(w[i][j]), from[(2 * (c * 16 + j * 4 + q) + (col >> 3)) * M + row], d, 0, 0, 0);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] += (float)s[e] * d[e];
+                        for (int e = 0; e < 4; ++e) sum[e] += (float)s[i][g][e] * d[e];
                     }
                 }
             }
@@ -217,14 +221,14 @@ __global__ void __launch_bounds__(W * 64) dense4_few_kernel(Dense a) {
     *reinterpret_cast<f4 *>(part + wave * 256 + col * 16 + 4 * q) = acc;
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * M; i += W * 64) {
-        const int m = i >> 4, n = n0 + (i & 15);
-        float s = 0.f;
+        const int r = i >> 4, n = n0 + (i & 15);
+        float y = 0.f;
         for (int k = 0; k < W; ++k) {
-            s += part[k * 256 + i];
-            if (!INT8) s += part[k * 256 + i + 128];
+            y += part[k * 256 + i];
+            if (!INT8) y += part[k * 256 + i + 128];
         }
-        if (INT8) s *= a.x_scale[m] * 0.0625f;
-        if (n < a.N) a.y[(uint64_t)m * a.N + n] = a.bias ? s + a.bias[n] : s;
+        if (INT8) y *= a.x_scale[r] * 0.0625f;
+        if (n < a.N) a.y[(uint64_t)r * a.N + n] = a.bias ? y + a.bias[n] : y;
     }
 }
 
