@@ -225,9 +225,9 @@ def test_refusals():
     with pytest.raises(NotImplementedError):
         F.dense_4bit(t(x, requires_grad=True), weight)
     need = be.lib.raw("xsmi_dense_4bit_workspace_bytes")
-    assert need(8, 64, 32, 32) == 0 and need(9, 64, 32, 32) > 0 and need(1 << 21, 64, 32, 32) == 0 and need(9, 64, 32, 16) == 0
-    y = be.empty((20, 32))
-    big = be.to_device(np.ones((20, 64), np.float32))
+    assert need(1, 64, 32, 32) == 0 and need(200, 64, 32, 32) > 0 and need(1 << 21, 64, 32, 32) == 0 and need(200, 64, 32, 16) == 0
+    y = be.empty((200, 32))
+    big = be.to_device(np.ones((200, 64), np.float32))
     for ws, size, codes in ((None, 0, weight.codes.ptr), (y.ptr, 16, weight.codes.ptr), (None, 0, None), (None, 0, weight.codes.ptr + 4)):
         with pytest.raises(ValueError):
-            be.lib.call("xsmi_dense_4bit", big.ptr, None, codes, weight.scales.ptr, None, y.ptr, 20, 64, 32, 32, ws, size)
+            be.lib.call("xsmi_dense_4bit", big.ptr, None, codes, weight.scales.ptr, None, y.ptr, 200, 64, 32, 32, ws, size)

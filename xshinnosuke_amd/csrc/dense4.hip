@@ -100,135 +100,228 @@ struct Dense {
 };
 
 // ---- few rows ----------------------------------------------------------------------------------------------------
-// A workgroup of W waves has 16 outputs and splits their inputs over its waves, chunk by chunk; the rows go through LDS, in
-// windows of W PF chunks, and the waves' sums are added at the end.  A float32 row takes two of the 16 columns of a multiplication, one for
-// each part (columns 0 to 7 the first parts, 8 to 15 the second), an 8-bit row one.  Columns without a row repeat the last
-// one: a column's sums are its own.  A window's loads are all under way before the first of them is needed: the rows' first, for
-// loads come back in order, then a wave's PF kilobytes of codes and their scales.
-template <int G, bool INT8, int W, int PF>
-__global__ void __launch_bounds__(W * 64) dense4_few_kernel(Dense a) {
+// All products are of 8-bit numbers here: weights times sixteen take three operations for eight of them, a quarter of what
+// float16 takes, and one row leaves that as the bound beside memory.  A float32 row becomes four rows of 8-bit digits: scaled by a
+// power of two to whole numbers below 2^30 and written in base 256 with signed digits, its sums are exact within a group and the
+// rows off by 2^-31 of the largest value at most.
+//
+// A workgroup of eight waves has 16 NT outputs and splits their inputs over its waves, chunk by chunk.  Each wave lays the rows'
+// part of its own PF chunks of a window out in its own stretch of LDS, by powers of two of its own, so that the waves meet
+// only where their sums are added at the end.  The loads of the next window are under way while one is multiplied.
+constexpr int WAVES = 8;
+
+// Eight whole numbers as four octets of digits, lowest first, in the order of weights_i8.
+__device__ __forceinline__ void digits8(const int *x, u2 *to) {
+    uint32_t y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = ((uint32_t)x[e] + 0x00808080u) ^ 0x00808080u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                    // numbers 0 2 4 6, then 1 3 5 7
+        const uint32_t a = __builtin_amdgcn_perm(y[2 + h], y[h], 0x05010400u), b = __builtin_amdgcn_perm(y[6 + h], y[4 + h], 0x05010400u);
+        const uint32_t c = __builtin_amdgcn_perm(y[2 + h], y[h], 0x07030602u), d = __builtin_amdgcn_perm(y[6 + h], y[4 + h], 0x07030602u);
+        to[0][h] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        to[1][h] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        to[2][h] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+        to[3][h] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+    }
+}
+
+// DIGITS 1: int8 rows, 4: float32 rows; CT tiles of 16 columns (a row and digit each), of which RPT octets a thread lays out.
+// Columns without a row repeat the last one: a column's sums are its own.  LOOP: there is more than one window.
+template <int G, int DIGITS, int CT, int NT, int PF, int RPT, bool LOOP>
+__global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ uint32_t most[W];
+    __shared__ int unusual[16];
     constexpr int GROUPS = 128 / G;                  // of a chunk
+    constexpr bool F32 = DIGITS == 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, col = lane & 15;
-    const int n0 = blockIdx.x * 16, M = a.M;
-    const u4 *const codes = reinterpret_cast<const u4 *>(a.codes) + (uint64_t)blockIdx.x * a.chunks * 64 + lane;
-    const _Float16 *const scales = a.scales + n0 + 4 * q;
-    const int row = INT8 ? min(col, M - 1) : min(col & 7, M - 1);
-    // float32 rows: W / width waves for each of up to `width` rows; a thread has up to MINE octets of one
-    constexpr int MINE = 4;
-    static_assert(INT8 || W == 8, "128 PF octets a row: 4 of each thread for PF 8, 4, 2 and width 2, 4, 8");
-    const int width = M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8, waves = W / width, m = wave / waves, mine = (wave % waves) * 64 + lane;
-    f4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first < a.chunks; first += W * PF) {
-        const int here = min(W * PF, a.chunks - first), octets = here * 16;
-        float v[MINE][8];
-        if (!INT8) {
+    const int M = a.M, R = M * DIGITS, tiles = a.cols / 16, t0 = blockIdx.x * NT;
+    if (F32 && threadIdx.x < 16) unusual[threadIdx.x] = 0;
+    if (F32) __syncthreads();
+    // A row's part of a window, 16 PF octets, is laid out by `share` lanes (float32: one row of a lane's own, so that the
+    // lanes of a row find its largest value together; int8: octets as they come).
+    const int width = !F32 || M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : M <= 8 ? 8 : 16, share = 64 / width, m = lane / share;
+    char *const mine = lds + wave * (PF * 128 * R);
+    const int first = wave, chunks = a.chunks;       // this wave's chunks: wave, wave + WAVES, ...
+    float xf[F32 ? RPT : 1][8];
+    i2 xi[F32 ? 1 : RPT];
+    u4 w[NT][PF];
+    h4 s[NT][PF][GROUPS];
+    // the octet of this thread's i-th in a window: row, chunk of the window, octet of the chunk
+    auto place = [&](int i, int &r, int &k, int &o) {
+        if (F32) {
+            const int p = lane % share + i * share;
+            r = m, k = p >> 4, o = p & 15;
+            return r < M && p < 16 * PF;
+        }
+        const int p = lane + i * 64;
+        r = p / (16 * PF), k = (p >> 4) % PF, o = p & 15;
+        return r < M;
+    };
+    auto load = [&](int c0) {
 #pragma unroll
-            for (int i = 0; i < MINE; ++i) {
-                const int o = mine + i * waves * 64;
-                if (m < M && o < octets) load8(static_cast<const float *>(a.x) + (uint64_t)m * a.K, first * 128 + o * 8, a.K, v[i]);
+        for (int i = 0; i < RPT; ++i) {
+            int r, k, o;
+            const bool live = place(i, r, k, o);
+            const int c = c0 + k * WAVES;
+            if (F32) {
+                if (live && c < chunks) load8(static_cast<const float *>(a.x) + (uint64_t)r * a.K, c * 128 + o * 8, a.K, xf[i]);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) xf[i][e] = 0.f;
+            } else {
+                xi[i] = i2{0, 0};
+                if (live && c < chunks) xi[i] = load8(static_cast<const int8_t *>(a.x) + (uint64_t)r * a.K, c * 128 + o * 8, a.K);
             }
-        } else {
-            u2 *const to = reinterpret_cast<u2 *>(lds);
-            for (int r = 0; r < M; ++r)
-                for (int o = threadIdx.x; o < octets; o += W * 64)
-                    to[o * M + r] = order_i8(load8(static_cast<const int8_t *>(a.x) + (uint64_t)r * a.K, first * 128 + o * 8, a.K));
         }
-        u4 w[PF];
-        h4 s[PF][GROUPS];
 #pragma unroll
-        for (int i = 0; i < PF; ++i) {
-            const int c = first + min(wave + W * i, here - 1);
-            w[i] = codes[(uint64_t)c * 64];
+        for (int t = 0; t < NT; ++t) {
+            const int tile = min(t0 + t, tiles - 1);
+            const u4 *const codes = reinterpret_cast<const u4 *>(a.codes) + (uint64_t)tile * chunks * 64 + lane;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) s[i][g] = *reinterpret_cast<const h4 *>(scales + (uint64_t)(c * GROUPS + g) * a.cols);
+            for (int i = 0; i < PF; ++i) {
+                const int c = min(c0 + i * WAVES, chunks - 1);       // a repeated chunk meets rows of zeros
+                w[t][i] = codes[(uint64_t)c * 64];
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) s[t][i][g] = *reinterpret_cast<const h4 *>(a.scales + (uint64_t)(c * GROUPS + g) * a.cols + tile * 16 + 4 * q);
+            }
         }
-        float back = 1.f;
-        if (!INT8) {
-            h8 *const to = reinterpret_cast<h8 *>(lds);
+    };
+    f4 acc[NT][CT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < CT; ++u) acc[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+    if (first < chunks) load(first);
+    for (int c0 = first; c0 < chunks; c0 += LOOP ? WAVES * PF : chunks) {
+        int exponent = 0;
+        if (F32) {
             uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < MINE; ++i)
-                if (m < M && mine + i * waves * 64 < octets)
+            for (int i = 0; i < RPT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = max(top, size_bits(v[i][e]));
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(xf[i][e]) & 0x7fffffffu);
+            if (top >= 0x7f800000u) {                // infinities and NaN are left to the end
+                top = 0;
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-            if (lane == 0) most[wave] = top;
-            __syncthreads();
-            uint32_t other = 0;
-            for (int k = 0; k < waves; ++k) {
-                top = max(top, most[m * waves + k]);
-                other = max(other, most[row * waves + k]);
+                for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (!(fabsf(xf[i][e]) < INFINITY)) xf[i][e] = 0.f;
+                        top = max(top, __float_as_uint(xf[i][e]) & 0x7fffffffu);
+                    }
+                unusual[m] = 1;
             }
-            back = scale_down(other);
-            const float up = scale_up(top);
+            for (int o = share / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+            exponent = (int)(top >> 23) - 156;       // values are below 2^(exponent + 30)
+        }
 #pragma unroll
-            for (int i = 0; i < MINE; ++i) {
-                const int o = mine + i * waves * 64;
-                if (m < M && o < octets) {
+        for (int i = 0; i < RPT; ++i) {
+            int r, k, o;
+            if (place(i, r, k, o)) {
+                // 16 bytes of a lane's operand hold octets o and o + 4 of eight
+                u2 *const to = reinterpret_cast<u2 *>(mine) + (((k * 2 + (o >> 3)) * 4 + (o & 3)) * R + r * DIGITS) * 2 + (o >> 2 & 1);
+                if (F32) {
+                    int n[8];
+                    u2 d[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][e] *= up;
-                    h8 hi, lo;
-                    split8(v[i], hi, lo);
-                    to[(2 * o) * M + m] = hi;
-                    to[(2 * o + 1) * M + m] = lo;
-                }
+                    for (int e = 0; e < 8; ++e) n[e] = __float2int_rn(ldexpf(xf[i][e], -exponent));
+                    digits8(n, d);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[2 * e] = d[e];
+                } else
+                    to[0] = order_i8(xi[i]);
             }
         }
-        __syncthreads();
-        f4 sum = {0.f, 0.f, 0.f, 0.f};
+        u4 wc[NT][PF];
+        h4 sc[NT][PF][GROUPS];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < PF; ++i) {
+                wc[t][i] = w[t][i];
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) sc[t][i][g] = s[t][i][g];
+            }
+        if (LOOP && c0 + WAVES * PF < chunks) load(c0 + WAVES * PF);
+        asm volatile("" ::: "memory");               // a wave's LDS operations stay in order
+        f4 sum[NT][CT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < CT; ++u) sum[t][u] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
-            const int c = wave + W * i;
-            if (c < here) {
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    if (INT8) {
-                        i4 d = {0, 0, 0, 0};
-                        const u2 *const from = reinterpret_cast<const u2 *>(lds);
+            for (int u = 0; u < CT; ++u) {
+                const int row = min(u * 16 + col, R - 1);
+                i4 x[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) x[j] = reinterpret_cast<const i4 *>(mine)[((i * 2 + j) * 4 + q) * R + row];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    i4 d = {0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const u2 lo = weights_i8(wc[t][i][2 * j]), hi = weights_i8(wc[t][i][2 * j + 1]);
                         if (G == 32) {
-                            const u2 wa = weights_i8(w[i][g]), xb = from[(c * 16 + g * 4 + q) * M + row];
-                            d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, wa), __builtin_bit_cast(long, xb), d, 0, 0, 0);
-                        } else {
+                            const i4 zero = {0, 0, 0, 0};
+                            const i4 e = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, lo), __builtin_bit_cast(long, i2{x[j].x, x[j].y}), zero, 0, 0, 0);
+                            const i4 f = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, hi), __builtin_bit_cast(long, i2{x[j].z, x[j].w}), zero, 0, 0, 0);
 #pragma unroll
-                            for (int j = g * (G / 32); j < (g + 1) * (G / 32); j += 2) {
-                                const u2 w0 = weights_i8(w[i][j]), w1 = weights_i8(w[i][j + 1]);
-                                const u2 x0 = from[(c * 16 + j * 4 + q) * M + row], x1 = from[(c * 16 + j * 4 + 4 + q) * M + row];
-                                d = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y},
-                                                                          i4{(int)x0.x, (int)x0.y, (int)x1.x, (int)x1.y}, d, 0, 0, 0);
+                            for (int v = 0; v < 4; ++v) {
+                                sum[t][u][v] += (float)sc[t][i][2 * j][v] * (float)e[v];
+                                sum[t][u][v] += (float)sc[t][i][2 * j + 1][v] * (float)f[v];
+                            }
+                        } else {
+                            d = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y}, x[j], d, 0, 0, 0);
+                            if (G == 64 || j == 1) {
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) sum[t][u][v] += (float)sc[t][i][G == 64 ? j : 0][v] * (float)d[v];
+                                d = i4{0, 0, 0, 0};
                             }
                         }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] += (float)s[i][g][e] * (float)d[e];
-                    } else {
-                        f4 d = {0.f, 0.f, 0.f, 0.f};
-                        const h8 *const from = reinterpret_cast<const h8 *>(lds);
-#pragma unroll
-                        for (int j = g * (G / 32); j < (g + 1) * (G / 32); ++j)
-                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(weights_f16(w[i][j]), from[(2 * (c * 16 + j * 4 + q) + (col >> 3)) * M + row], d, 0, 0, 0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[e] += (float)s[i][g][e] * d[e];
                     }
                 }
             }
         }
-        acc += sum * back;                           // a window has its own power of two
-        __syncthreads();
-    }
-    float *const part = reinterpret_cast<float *>(lds);      // [wave][column][output]
-    *reinterpret_cast<f4 *>(part + wave * 256 + col * 16 + 4 * q) = acc;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * M; i += W * 64) {
-        const int r = i >> 4, n = n0 + (i & 15);
-        float y = 0.f;
-        for (int k = 0; k < W; ++k) {
-            y += part[k * 256 + i];
-            if (!INT8) y += part[k * 256 + i + 128];
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < CT; ++u) {
+            // a column's digit, the sixteen in its weights, and its row's power of two in this wave and window
+            const int row = min(u * 16 + col, R - 1);
+            const int e = F32 ? __shfl(exponent, row / 4 * share) + 8 * (row & 3) - 4 : -4;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) acc[t][u][v] += ldexpf(sum[t][u][v], e);
         }
-        if (INT8) y *= a.x_scale[r] * 0.0625f;
-        if (n < a.N) a.y[(uint64_t)r * a.N + n] = a.bias ? y + a.bias[n] : y;
+    }
+    __syncthreads();
+    float *const part = reinterpret_cast<float *>(lds);      // [wave][tile of outputs][column][output]
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < CT; ++u) *reinterpret_cast<f4 *>(part + (((wave * NT + t) * CT + u) * 16 + col) * 16 + 4 * q) = acc[t][u];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * NT * M; i += WAVES * 64) {
+        const int r = i / (16 * NT), t = i / 16 % NT, n = (t0 + t) * 16 + (i & 15);
+        if (n >= a.N) continue;
+        float y = 0.f;
+        for (int k = 0; k < WAVES; ++k)
+#pragma unroll
+            for (int e = DIGITS - 1; e >= 0; --e) y += part[((k * NT + t) * CT * 16 + r * DIGITS + e) * 16 + (i & 15)];
+        if (!F32) y *= a.x_scale[r];
+        if (F32 && unusual[r]) {                     // what is not finite decides; one thread goes through the row
+            const float *const x = static_cast<const float *>(a.x) + (uint64_t)r * a.K;
+            for (int k = 0; k < a.K; ++k)
+                if (!(fabsf(x[k]) < INFINITY)) {
+                    const int in = k & 127;
+                    const uint8_t b = a.codes[(((uint64_t)(n >> 4) * chunks + (k >> 7)) * 64 + 16 * (in % 32 / 8) + (n & 15)) * 16 + 4 * (in / 32) + in % 8 / 2];
+                    y += x[k] * ((float)((int)((k & 1 ? b >> 4 : b & 15) ^ 8) - 8) * (float)a.scales[(uint64_t)(k / G) * a.cols + n]);
+                }
+        }
+        a.y[(uint64_t)r * a.N + n] = a.bias ? y + a.bias[n] : y;
     }
 }
 
@@ -393,25 +486,46 @@ int check_weights(const char *who, int K, int N, int group) {
     return XSMI_OK;
 }
 
-// Few rows: those that fit the columns of one multiplication.
-inline bool few(size_t M, bool int8) { return M <= (int8 ? 16u : 8u); }
+// Few rows: those whose digits fit four tiles of columns.
+inline bool few(size_t M, bool int8) { return M <= (int8 ? 64u : 16u); }
 
-template <int G, bool INT8, int PF>
+// ROWS: the most that there may be.
+template <int G, int DIGITS, int ROWS, int NT, int PF, bool LOOP>
 int launch_few(const Dense &a) {
-    constexpr int W = 8;
-    const int window = a.chunks < W * PF ? a.chunks : W * PF;
-    const size_t rows = (size_t)window * 128 * a.M * (INT8 ? 1 : 4), sums = W * 1024, bytes = rows > sums ? rows : sums;
-    hipLaunchKernelGGL((dense4_few_kernel<G, INT8, W, PF>), dim3(a.cols / 16), dim3(W * 64), bytes, xsmi::stream(), a);
+    constexpr int CT = (ROWS * DIGITS + 15) / 16, LAID = DIGITS == 4 && ROWS == 12 ? 16 : ROWS, RPT = PF * LAID < 4 ? 1 : PF * LAID / 4;
+    const size_t rows = (size_t)WAVES * PF * 128 * a.M * DIGITS, sums = (size_t)WAVES * NT * CT * 1024, bytes = rows > sums ? rows : sums;
+    hipLaunchKernelGGL((dense4_few_kernel<G, DIGITS, CT, NT, PF, RPT, LOOP>), dim3((a.cols / 16 + NT - 1) / NT), dim3(WAVES * 64), bytes, xsmi::stream(), a);
     XSMI_LAUNCH_CHECK("dense4_few_kernel");
     return XSMI_OK;
 }
 
+// One window where a wave's chunks fit one, and 64 KB of LDS.
+template <int G, int DIGITS>
+int launch_few(const Dense &a) {
+    constexpr int FULL = 16 / DIGITS;                // rows of a tile of columns
+    const int R = a.M * DIGITS, each = (a.chunks + WAVES - 1) / WAVES;
+    if (a.M == 1) {
+        if (each <= 1) return launch_few<G, DIGITS, 1, 1, 1, false>(a);
+        if (each <= 2) return launch_few<G, DIGITS, 1, 1, 2, false>(a);
+        if (each <= 4) return launch_few<G, DIGITS, 1, 1, 4, false>(a);
+        if (each <= 8) return launch_few<G, DIGITS, 1, 1, 8, false>(a);
+        return launch_few<G, DIGITS, 1, 1, 4, true>(a);
+    }
+    if (R <= 16) {
+        if (each <= 1) return launch_few<G, DIGITS, FULL, 1, 1, false>(a);
+        if (each <= 2) return launch_few<G, DIGITS, FULL, 1, 2, false>(a);
+        if (each <= 4) return launch_few<G, DIGITS, FULL, 1, 4, false>(a);
+        return launch_few<G, DIGITS, FULL, 1, 4, true>(a);
+    }
+    if (R <= 32) return launch_few<G, DIGITS, 2 * FULL, 2, 2, true>(a);
+    // (three tiles of float32 rows are up to twelve, which lay out as sixteen)
+    if (R <= 48) return launch_few<G, DIGITS, 3 * FULL, 2, 1, true>(a);
+    return launch_few<G, DIGITS, 4 * FULL, 2, 1, true>(a);
+}
+
 template <int G, bool INT8>
 int launch(const Dense &a, void *ws) {
-    if (few(a.M, INT8)) {
-        const int rows = INT8 ? (a.M + 3) / 4 : a.M;         // windows of 64 KB at most
-        return rows <= 2 ? launch_few<G, INT8, 8>(a) : rows <= 4 ? launch_few<G, INT8, 4>(a) : launch_few<G, INT8, 2>(a);
-    }
+    if (few(a.M, INT8)) return launch_few<G, INT8 ? 1 : 4>(a);
     const int tiles = up(a.M, 16) / 16;
     float *const back = (float *)ws;
     void *const operand = (char *)ws + up(a.M, 64) * 4;
