@@ -27,12 +27,14 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 // Eight weights as float16, in the order 0 4 1 5 2 6 3 7: with the sign turned into an offset a code's four bits are the low
 // bits of the float16 1024 + c + 8, or, four places up, of 64 + c + 8; taking 1032 or 72 off is exact.
 __device__ __forceinline__ h8 weights_f16(uint32_t w) {
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, at10 = 0x64006400u, at6 = 0x54005400u;
+    asm("" : "+s"(low), "+s"(high), "+s"(at10), "+s"(at6));      // registers: one instruction takes no two constants of 32 bits
     const uint32_t u = w ^ 0x88888888u, v = u >> 8;
     const h2 far = {(_Float16)1032.f, (_Float16)1032.f}, near = {(_Float16)72.f, (_Float16)72.f};
-    const h2 a = __builtin_bit_cast(h2, (u & 0x000f000fu) | 0x64006400u) - far;
-    const h2 b = __builtin_bit_cast(h2, (u & 0x00f000f0u) | 0x54005400u) - near;
-    const h2 c = __builtin_bit_cast(h2, (v & 0x000f000fu) | 0x64006400u) - far;
-    const h2 d = __builtin_bit_cast(h2, (v & 0x00f000f0u) | 0x54005400u) - near;
+    const h2 a = __builtin_bit_cast(h2, (u & low) | at10) - far;
+    const h2 b = __builtin_bit_cast(h2, (u & high) | at6) - near;
+    const h2 c = __builtin_bit_cast(h2, (v & low) | at10) - far;
+    const h2 d = __builtin_bit_cast(h2, (v & high) | at6) - near;
     return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
@@ -326,16 +328,26 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------------------
-// The rows laid out first as the matrix instructions read them: [32 inputs][16 rows][part][lane], a lane's octet of one row.
+// The rows are laid out first as the matrix instructions read them, for each 64 rows and chunk of 128 inputs in one piece:
+// float32 [step of 32 inputs][tile of 16 rows][part][lane], a lane's octet of one row as float16; int8 [64 inputs][tile][lane][octets o and o + 4].
 // One workgroup a row.  Rows behind the last one are not written: a column's sums are its own.
+constexpr int BLOCK_ROWS = 64;
+constexpr uint32_t piece_bytes(bool int8) { return int8 ? 64 * 128 : 64 * 128 * 4; }
+constexpr int many_stages(bool int8) { return int8 ? 5 : 3; }
+constexpr uint32_t many_lds_bytes(bool int8) { return many_stages(int8) * (piece_bytes(int8) + 9 * 1024); }
+
 template <bool INT8>
-__global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, void *operand, float *back, int tiles) {
+__global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, char *operand, float *back) {
     __shared__ uint32_t most[4];
-    const int m = blockIdx.x, octets = a.chunks * 16;
+    const int m = blockIdx.x, octets = a.chunks * 16, in = m & 63;
+    char *const block = operand + (uint64_t)(m >> 6) * a.chunks * piece_bytes(INT8);
     if (INT8) {
-        u2 *const to = static_cast<u2 *>(operand);
-        for (int o = threadIdx.x; o < octets; o += 256)
-            to[((uint64_t)(o >> 2) * tiles + (m >> 4)) * 64 + (o & 3) * 16 + (m & 15)] = order_i8(load8(static_cast<const int8_t *>(a.x) + (uint64_t)m * a.K, o * 8, a.K));
+        const int8_t *const x = static_cast<const int8_t *>(a.x) + (uint64_t)m * a.K;
+        for (int o = threadIdx.x; o < octets; o += 256) {
+            const int k = o & 15;
+            u2 *const to = reinterpret_cast<u2 *>(block + (uint64_t)(o >> 4) * piece_bytes(true)) + (((k >> 3) * 4 + (in >> 4)) * 64 + (k & 3) * 16 + (in & 15)) * 2 + (k >> 2 & 1);
+            *to = order_i8(load8(x, o * 8, a.K));
+        }
         return;
     }
     const float *const x = static_cast<const float *>(a.x) + (uint64_t)m * a.K;
@@ -353,7 +365,6 @@ __global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, void *operand
     top = max(max(most[0], most[1]), max(most[2], most[3]));
     if (threadIdx.x == 0) back[m] = scale_down(top);
     const float up = scale_up(top);
-    h8 *const to = static_cast<h8 *>(operand);
     for (int o = threadIdx.x; o < octets; o += 256) {
         float v[8];
         load8(x, o * 8, a.K, v);
@@ -361,77 +372,154 @@ __global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, void *operand
         for (int e = 0; e < 8; ++e) v[e] *= up;
         h8 hi, lo;
         split8(v, hi, lo);
-        const uint64_t at = (((uint64_t)(o >> 2) * tiles + (m >> 4)) * 2) * 64 + (o & 3) * 16 + (m & 15);
-        to[at] = hi;
-        to[at + 64] = lo;
+        const int k = o & 15;
+        h8 *const to = reinterpret_cast<h8 *>(block + (uint64_t)(o >> 4) * piece_bytes(false)) + ((k >> 2) * 4 + (in >> 4)) * 128 + (k & 3) * 16 + (in & 15);
+        to[0] = hi;
+        to[64] = lo;
     }
 }
 
-// A wave has 16 outputs and MT tiles of 16 rows, a workgroup four waves of the same rows.
-template <int G, bool INT8, int MT>
-__global__ void __launch_bounds__(256) dense4_many_kernel(Dense a, const void *operand, const float *back, int tiles) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, col = lane & 15;
-    const int tile = blockIdx.x * 4 + wave, n0 = tile * 16, t0 = blockIdx.y * MT;
-    if (n0 >= a.cols) return;
-    const u4 *const codes = reinterpret_cast<const u4 *>(a.codes) + (uint64_t)tile * a.chunks * 64 + lane;
-    const _Float16 *const scales = a.scales + n0 + 4 * q;
-    f4 acc[MT];
+// A workgroup of eight waves has 128 outputs and 64 rows, a wave 64 of the outputs, 32 of the rows and one half of each chunk's
+// inputs (one wave for both halves leaves its SIMD idle two thirds of the time: 200 rows, 4096 x 8192 took 54 us).  Rows, codes and scales of a
+// chunk are loaded straight into one of a ring of stages in LDS, STAGES - 1 chunks ahead of the one that is multiplied: one
+// workgroup a compute unit has nobody else to hide a load behind.
+template <int G, bool INT8>
+__global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char *operand, const float *back) {
+    constexpr uint32_t ROWS = piece_bytes(INT8), CODES = 8 * 1024, SCALES = 1024, STAGE = ROWS + CODES + SCALES;
+    constexpr int STAGES = many_stages(INT8), LOADS = ROWS / 8192 + CODES / 8192 + 1;       // of a wave for a chunk
+    constexpr int GROUPS = 128 / G, NT = 4, MT = 2;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, col = lane & 15;
+    const int tiles = a.cols / 16, t0 = blockIdx.x * 8, n_wave = (wave & 1) * NT, u0 = (wave >> 1 & 1) * MT, half = wave >> 2;
+    const char *const block = operand + (uint64_t)blockIdx.y * a.chunks * ROWS;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)&lds[0];
+    // scales: 16 lanes for the 256 bytes of a group's 128 outputs; what lies behind the row of scales reads as zero
+    const uint32_t row_bytes = (uint32_t)min(256, (a.cols - t0 * 16) * 2);
+    auto issue = [&](int c) {
+        const uint32_t to = lds0 + (uint32_t)(c % STAGES) * STAGE;
+        const xsmi::xsmi_int32x4 rows = xsmi::make_rsrc(block + (uint64_t)c * ROWS, ROWS);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t i = 0; i < ROWS / 8192; ++i) {
+            const uint32_t at = (i * 8 + wave) * 1024;
+            xsmi::load_lds_b128(rows, to + at, at + lane * 16, 0);
+        }
+        const xsmi::xsmi_int32x4 codes = xsmi::make_rsrc(a.codes + ((uint64_t)min(t0 + wave, tiles - 1) * a.chunks + c) * 1024, 1024);
+        xsmi::load_lds_b128(codes, to + ROWS + wave * 1024, lane * 16, 0);
+        // group (lane >> 4) of the chunk; the same by every wave, so that all have as many loads under way
+        const xsmi::xsmi_int32x4 scales = xsmi::make_rsrc(a.scales + (uint64_t)c * GROUPS * a.cols + t0 * 16, (uint32_t)(GROUPS - 1) * a.cols * 2 + row_bytes);
+        const uint32_t in = (uint32_t)(lane & 15) * 16;
+        xsmi::load_lds_b128(scales, to + ROWS + CODES, (lane >> 4) < GROUPS && in < row_bytes ? (uint32_t)(lane >> 4) * a.cols * 2 + in : 0x80000000u, 0);
+    };
+    f4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < STAGES - 1; ++c)
+        if (c < a.chunks) issue(c);
     for (int c = 0; c < a.chunks; ++c) {
-        const u4 w = codes[(uint64_t)c * 64];
+        // this wave's part of the chunk has arrived when no more than the later chunks' loads are under way
+        if (c + STAGES - 1 <= a.chunks) xsmi::wait_vmcnt<LOADS * (STAGES - 2)>(); else xsmi::wait_vmcnt<0>();
+        xsmi::block_barrier();                       // everybody's has; and the chunk before this one has been read
+        if (c + STAGES - 1 < a.chunks) issue(c + STAGES - 1);
+        const char *const stage = lds + (uint32_t)(c % STAGES) * STAGE;
+        u2 wc[NT];                                   // steps 2 half and 2 half + 1
 #pragma unroll
-        for (int g = 0; g < 128 / G; ++g) {
-            const h4 s = *reinterpret_cast<const h4 *>(scales + (uint64_t)(c * (128 / G) + g) * a.cols);
-            if (INT8) {
-                const u2 *const from = static_cast<const u2 *>(operand) + lane;
-                i4 d[MT];
+        for (int t = 0; t < NT; ++t) wc[t] = reinterpret_cast<const u2 *>(stage + ROWS)[((n_wave + t) * 64 + lane) * 2 + half];
+        auto scale = [&](int t, int step) {
+            return *reinterpret_cast<const h4 *>(stage + ROWS + CODES + (2 * half + step) / (G / 32) * 256 + (n_wave + t) * 32 + q * 8);
+        };
+        if (INT8) {
+            i4 x[MT];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) d[t] = i4{0, 0, 0, 0};
+            for (int u = 0; u < MT; ++u) x[u] = reinterpret_cast<const i4 *>(stage)[(half * 4 + u0 + u) * 64 + lane];
 #pragma unroll
-                for (int j = g * (G / 32); j < (g + 1) * (G / 32); ++j) {
-                    const long wa = __builtin_bit_cast(long, weights_i8(w[j]));
+            for (int t = 0; t < NT; ++t) {
+                const u2 lo = weights_i8(wc[t].x), hi = weights_i8(wc[t].y);
+                const h4 s0 = scale(t, 0), s1 = scale(t, 1);
+                const i4 zero = {0, 0, 0, 0};
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        const u2 x = from[((uint64_t)(c * 4 + j) * tiles + min(t0 + t, tiles - 1)) * 64];
-                        d[t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(wa, __builtin_bit_cast(long, x), d[t], 0, 0, 0);
+                for (int u = 0; u < MT; ++u) {
+                    if (G == 32) {
+                        const i4 e = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, lo), __builtin_bit_cast(long, i2{x[u].x, x[u].y}), zero, 0, 0, 0);
+                        const i4 f = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, hi), __builtin_bit_cast(long, i2{x[u].z, x[u].w}), zero, 0, 0, 0);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)s0[v] * (float)e[v] + (float)s1[v] * (float)f[v];
+                    } else {
+                        const i4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y}, x[u], zero, 0, 0, 0);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)s0[v] * (float)d[v];
                     }
                 }
+            }
+        } else {
+            f4 d[NT][MT];
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
+            for (int j = 0; j < 2; ++j) {
+                h8 x[2][MT];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][e] += (float)s[e] * (float)d[t][e];
-            } else {
-                const h8 *const from = static_cast<const h8 *>(operand) + lane;
-                f4 d[MT];
+                for (int u = 0; u < MT; ++u)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) d[t] = f4{0.f, 0.f, 0.f, 0.f};
+                    for (int p = 0; p < 2; ++p) x[p][u] = reinterpret_cast<const h8 *>(stage)[(((2 * half + j) * 4 + u0 + u) * 2 + p) * 64 + lane];
+                h8 wa[NT];
 #pragma unroll
-                for (int j = g * (G / 32); j < (g + 1) * (G / 32); ++j) {
-                    const h8 wa = weights_f16(w[j]);
+                for (int t = 0; t < NT; ++t) wa[t] = weights_f16(j ? wc[t].y : wc[t].x);
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        const h8 *const x = from + ((uint64_t)(c * 4 + j) * tiles + min(t0 + t, tiles - 1)) * 128;
-                        d[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, x[0], d[t], 0, 0, 0);
-                        d[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, x[64], d[t], 0, 0, 0);
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int u = 0; u < MT; ++u) {
+                            const f4 from = p == 0 && (G == 32 || j == 0) ? f4{0.f, 0.f, 0.f, 0.f} : d[t][u];
+                            d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa[t], x[p][u], from, 0, 0, 0);
+                        }
+                if (G == 32 || j == 1) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const h4 s = scale(t, j);
+#pragma unroll
+                        for (int u = 0; u < MT; ++u)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)s[v] * d[t][u][v];
                     }
                 }
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][e] += (float)s[e] * d[t][e];
             }
         }
     }
+    // the halves' sums: those of the second through LDS to the waves of the first
+    __syncthreads();
+    f4 *const other = reinterpret_cast<f4 *>(lds) + ((wave & 3) * NT * MT) * 64 + lane;
+    if (half) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = (t0 + t) * 16 + col;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < MT; ++u) other[(t * MT + u) * 64] = acc[t][u];
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[t][u] += other[(t * MT + u) * 64];
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+        const int m = blockIdx.y * BLOCK_ROWS + (u0 + u) * 16 + col;
         if (m >= a.M) continue;
         const float f = INT8 ? a.x_scale[m] * 0.0625f : back[m];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int n = n0 + 4 * q + e;
-            if (n < a.N) a.y[(uint64_t)m * a.N + n] = acc[t][e] * f + (a.bias ? a.bias[n] : 0.f);
+        for (int t = 0; t < NT; ++t) {
+            const int n = (t0 + n_wave + t) * 16 + 4 * q;
+            f4 y = acc[t][u] * f;
+            float *const to = a.y + (uint64_t)m * a.N + n;
+            if (n + 4 <= a.N) {
+                if (a.bias) y += *reinterpret_cast<const f4u *>(a.bias + n);
+                *reinterpret_cast<f4u *>(to) = y;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) to[e] = a.bias ? y[e] + a.bias[n + e] : y[e];
+            }
         }
     }
 }
@@ -477,7 +565,6 @@ __global__ void __launch_bounds__(256) dequantize4_kernel(const uint8_t *__restr
     w[i] = (float)c * (float)scales[(uint64_t)(k / group) * cols + n];
 }
 
-constexpr int ROW_TILES = 4;                         // of 16 rows: of a workgroup of dense4_many_kernel
 inline int up(int v, int to) { return (v + to - 1) / to * to; }
 
 int check_weights(const char *who, int K, int N, int group) {
@@ -526,13 +613,12 @@ int launch_few(const Dense &a) {
 template <int G, bool INT8>
 int launch(const Dense &a, void *ws) {
     if (few(a.M, INT8)) return launch_few<G, INT8 ? 1 : 4>(a);
-    const int tiles = up(a.M, 16) / 16;
     float *const back = (float *)ws;
-    void *const operand = (char *)ws + up(a.M, 64) * 4;
-    hipLaunchKernelGGL(dense4_rows_kernel<INT8>, dim3(a.M), dim3(256), 0, xsmi::stream(), a, operand, back, tiles);
+    char *const operand = (char *)ws + up(a.M, BLOCK_ROWS) * 4;
+    hipLaunchKernelGGL(dense4_rows_kernel<INT8>, dim3(a.M), dim3(256), 0, xsmi::stream(), a, operand, back);
     XSMI_LAUNCH_CHECK("dense4_rows_kernel");
-    hipLaunchKernelGGL((dense4_many_kernel<G, INT8, ROW_TILES>), dim3((a.cols / 16 + 3) / 4, (tiles + ROW_TILES - 1) / ROW_TILES), dim3(256), 0, xsmi::stream(), a,
-                       (const void *)operand, (const float *)back, tiles);
+    hipLaunchKernelGGL((dense4_many_kernel<G, INT8>), dim3((a.cols + 127) / 128, (a.M + BLOCK_ROWS - 1) / BLOCK_ROWS), dim3(512), many_lds_bytes(INT8), xsmi::stream(),
+                       a, (const char *)operand, (const float *)back);
     XSMI_LAUNCH_CHECK("dense4_many_kernel");
     return XSMI_OK;
 }
@@ -553,7 +639,7 @@ size_t xsmi_dense_4bit_scale_count(int K, int N, int group) {
 
 size_t xsmi_dense_4bit_workspace_bytes(size_t M, int K, int N, int x_bits) {
     if (K < 1 || N < 1 || K > (1 << 30) || N > (1 << 30) || (x_bits != 8 && x_bits != 32) || M >= (1u << 21) || few(M, x_bits == 8)) return 0;
-    return (size_t)up((int)M, 64) * 4 + (size_t)up((int)M, 16) * up(K, 128) * (x_bits == 8 ? 1 : 4);
+    return (size_t)up((int)M, BLOCK_ROWS) * (4 + (size_t)up(K, 128) * (x_bits == 8 ? 1 : 4));
 }
 
 int xsmi_quantize_4bit(const float *w, int K, int N, int group, uint8_t *codes, void *scales) {
