@@ -379,24 +379,25 @@ __global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, char *operand
     }
 }
 
-// A workgroup of eight waves has 128 outputs and 64 rows, a wave 64 of the outputs, 32 of the rows and one half of each chunk's
-// inputs (one wave for both halves leaves its SIMD idle two thirds of the time: 200 rows, 4096 x 8192 took 54 us).  Rows, codes and scales of a
-// chunk are loaded straight into one of a ring of stages in LDS, STAGES - 1 chunks ahead of the one that is multiplied: one
-// workgroup a compute unit has nobody else to hide a load behind.
+// A workgroup of eight waves has 128 outputs and 64 rows, a wave 32 of the outputs, all the rows and one half of each chunk's
+// inputs.  Rows, codes and scales of a chunk are loaded straight into one of a ring of stages in LDS, STAGES - 1 chunks
+// ahead of the one that is multiplied, and a step's operands are read from there while the step before it is multiplied: one workgroup a
+// compute unit has nobody else to hide a wait behind.  Each weight is turned into float16 by one wave only, for 64 rows: that takes
+// the vector unit as long as the multiplications take the matrix unit where two waves do it for 32 rows each.
 template <int G, bool INT8>
 __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char *operand, const float *back) {
     constexpr uint32_t ROWS = piece_bytes(INT8), CODES = 8 * 1024, SCALES = 1024, STAGE = ROWS + CODES + SCALES;
     constexpr int STAGES = many_stages(INT8), LOADS = ROWS / 8192 + CODES / 8192 + 1;       // of a wave for a chunk
-    constexpr int GROUPS = 128 / G, NT = 4, MT = 2;
+    constexpr int GROUPS = 128 / G, NT = 2, MT = 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, col = lane & 15;
-    const int tiles = a.cols / 16, t0 = blockIdx.x * 8, n_wave = (wave & 1) * NT, u0 = (wave >> 1 & 1) * MT, half = wave >> 2;
+    const int tiles = a.cols / 16, t0 = blockIdx.x * 8, n_wave = (wave & 3) * NT, half = wave >> 2;
     const char *const block = operand + (uint64_t)blockIdx.y * a.chunks * ROWS;
     const uint32_t lds0 = (uint32_t)(uintptr_t)&lds[0];
     // scales: 16 lanes for the 256 bytes of a group's 128 outputs; what lies behind the row of scales reads as zero
     const uint32_t row_bytes = (uint32_t)min(256, (a.cols - t0 * 16) * 2);
-    auto issue = [&](int c) {
-        const uint32_t to = lds0 + (uint32_t)(c % STAGES) * STAGE;
+    auto issue = [&](int c, int at_stage) {
+        const uint32_t to = lds0 + (uint32_t)at_stage * STAGE;
         const xsmi::xsmi_int32x4 rows = xsmi::make_rsrc(block + (uint64_t)c * ROWS, ROWS);
 #pragma unroll
         for (uint32_t i = 0; i < ROWS / 8192; ++i) {
@@ -410,82 +411,122 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
         const uint32_t in = (uint32_t)(lane & 15) * 16;
         xsmi::load_lds_b128(scales, to + ROWS + CODES, (lane >> 4) < GROUPS && in < row_bytes ? (uint32_t)(lane >> 4) * a.cols * 2 + in : 0x80000000u, 0);
     };
+    // what a wave multiplies of a chunk: steps 2 half and 2 half + 1 of codes, their scales; rows a step at a time
+    constexpr int OWN = GROUPS == 4 ? 2 : 1;
+    struct Weights {
+        u2 w[NT];
+        h4 s[NT][OWN];
+    };
+    auto read_weights = [&](const char *stage, Weights &r) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            r.w[t] = reinterpret_cast<const u2 *>(stage + ROWS)[((n_wave + t) * 64 + lane) * 2 + half];
+#pragma unroll
+            for (int g = 0; g < OWN; ++g)
+                r.s[t][g] = *reinterpret_cast<const h4 *>(stage + ROWS + CODES + (2 * half + g) / (G / 32) * 256 + (n_wave + t) * 32 + q * 8);
+        }
+    };
+    struct Rows {
+        u4 x[INT8 ? 1 : 2][MT];
+    };
+    auto read_rows = [&](const char *stage, int step, Rows &r) {
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+#pragma unroll
+            for (int p = 0; p < (INT8 ? 1 : 2); ++p)
+                r.x[p][u] = reinterpret_cast<const u4 *>(stage)[INT8 ? (half * 4 + u) * 64 + lane : (((2 * half + step) * 4 + u) * 2 + p) * 64 + lane];
+    };
     f4 acc[NT][MT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int u = 0; u < MT; ++u) acc[t][u] = f4{0.f, 0.f, 0.f, 0.f};
+    f4 d[NT][MT];
+    auto multiply_f16 = [&](const Weights &r, const Rows &x, int step) {
+        h8 w[NT];
 #pragma unroll
-    for (int c = 0; c < STAGES - 1; ++c)
-        if (c < a.chunks) issue(c);
-    for (int c = 0; c < a.chunks; ++c) {
-        // this wave's part of the chunk has arrived when no more than the later chunks' loads are under way
-        if (c + STAGES - 1 <= a.chunks) xsmi::wait_vmcnt<LOADS * (STAGES - 2)>(); else xsmi::wait_vmcnt<0>();
-        xsmi::block_barrier();                       // everybody's has; and the chunk before this one has been read
-        if (c + STAGES - 1 < a.chunks) issue(c + STAGES - 1);
-        const char *const stage = lds + (uint32_t)(c % STAGES) * STAGE;
-        u2 wc[NT];                                   // steps 2 half and 2 half + 1
+        for (int t = 0; t < NT; ++t) w[t] = weights_f16(step ? r.w[t].y : r.w[t].x);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) wc[t] = reinterpret_cast<const u2 *>(stage + ROWS)[((n_wave + t) * 64 + lane) * 2 + half];
-        auto scale = [&](int t, int step) {
-            return *reinterpret_cast<const h4 *>(stage + ROWS + CODES + (2 * half + step) / (G / 32) * 256 + (n_wave + t) * 32 + q * 8);
-        };
-        if (INT8) {
-            i4 x[MT];
+        for (int p = 0; p < 2; ++p)
 #pragma unroll
-            for (int u = 0; u < MT; ++u) x[u] = reinterpret_cast<const i4 *>(stage)[(half * 4 + u0 + u) * 64 + lane];
+            for (int u = 0; u < MT; ++u)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const u2 lo = weights_i8(wc[t].x), hi = weights_i8(wc[t].y);
-                const h4 s0 = scale(t, 0), s1 = scale(t, 1);
-                const i4 zero = {0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < MT; ++u) {
-                    if (G == 32) {
-                        const i4 e = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, lo), __builtin_bit_cast(long, i2{x[u].x, x[u].y}), zero, 0, 0, 0);
-                        const i4 f = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, hi), __builtin_bit_cast(long, i2{x[u].z, x[u].w}), zero, 0, 0, 0);
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)s0[v] * (float)e[v] + (float)s1[v] * (float)f[v];
-                    } else {
-                        const i4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y}, x[u], zero, 0, 0, 0);
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)s0[v] * (float)d[v];
-                    }
+                for (int t = 0; t < NT; ++t) {
+                    const f4 from = p == 0 && (G == 32 || step == 0) ? f4{0.f, 0.f, 0.f, 0.f} : d[t][u];
+                    d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[t], __builtin_bit_cast(h8, x.x[INT8 ? 0 : p][u]), from, 0, 0, 0);
                 }
-            }
-        } else {
-            f4 d[NT][MT];
+        if (G == 32 || step == 1) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                h8 x[2][MT];
+            for (int u = 0; u < MT; ++u)
 #pragma unroll
-                for (int u = 0; u < MT; ++u)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) x[p][u] = reinterpret_cast<const h8 *>(stage)[(((2 * half + j) * 4 + u0 + u) * 2 + p) * 64 + lane];
-                h8 wa[NT];
+                    for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)r.s[t][step % OWN][v] * d[t][u][v];
+        }
+    };
+    auto multiply_i8 = [&](const Weights &r, const Rows &x) {
+        const i4 zero = {0, 0, 0, 0};
 #pragma unroll
-                for (int t = 0; t < NT; ++t) wa[t] = weights_f16(j ? wc[t].y : wc[t].x);
+        for (int t = 0; t < NT; ++t) {
+            const u2 lo = weights_i8(r.w[t].x), hi = weights_i8(r.w[t].y);
 #pragma unroll
-                for (int p = 0; p < 2; ++p)
+            for (int u = 0; u < MT; ++u) {
+                const u4 b = x.x[0][u];
+                if (G == 32) {
+                    const i4 e = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, lo), __builtin_bit_cast(long, u2{b.x, b.y}), zero, 0, 0, 0);
+                    const i4 f = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, hi), __builtin_bit_cast(long, u2{b.z, b.w}), zero, 0, 0, 0);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int u = 0; u < MT; ++u) {
-                            const f4 from = p == 0 && (G == 32 || j == 0) ? f4{0.f, 0.f, 0.f, 0.f} : d[t][u];
-                            d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa[t], x[p][u], from, 0, 0, 0);
-                        }
-                if (G == 32 || j == 1) {
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const h4 s = scale(t, j);
-#pragma unroll
-                        for (int u = 0; u < MT; ++u)
-#pragma unroll
-                            for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)s[v] * d[t][u][v];
+                    for (int v = 0; v < 4; ++v) {
+                        acc[t][u][v] += (float)r.s[t][0][v] * (float)e[v];
+                        acc[t][u][v] += (float)r.s[t][OWN - 1][v] * (float)f[v];
                     }
+                } else {
+                    const i4 e = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y}, __builtin_bit_cast(i4, b), zero, 0, 0, 0);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)r.s[t][0][v] * (float)e[v];
                 }
             }
         }
+    };
+    // A chunk can be read once this wave's loads of it have arrived (no more than the later chunks' are under way) and, behind
+    // the barrier, everybody's have; the chunk before it has been read by then: its stage is loaded anew after that.
+    auto arrive = [&](int c) {
+        if (c + STAGES - 1 <= a.chunks) xsmi::wait_vmcnt<LOADS * (STAGES - 2)>(); else xsmi::wait_vmcnt<0>();
+        xsmi::wait_lgkmcnt0();
+        xsmi::block_barrier();
+    };
+#pragma unroll
+    for (int c = 0; c < STAGES - 1; ++c)
+        if (c < a.chunks) issue(c, c);
+    Weights w;
+    Rows x;
+    arrive(0);
+    read_weights(lds, w);
+    read_rows(lds, 0, x);
+    int stage = 0;
+    for (int c = 0; c < a.chunks; ++c) {
+        const int after = stage + 1 == STAGES ? 0 : stage + 1;
+        const bool more = c + 1 < a.chunks;
+        if (c + STAGES - 1 < a.chunks) issue(c + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);      // where chunk c - 1 was
+        Weights w1;
+        Rows x1;
+        if (!INT8) {
+            read_rows(lds + (uint32_t)stage * STAGE, 1, x1);
+            multiply_f16(w, x, 0);
+        }
+        if (more) {
+            arrive(c + 1);
+            read_weights(lds + (uint32_t)after * STAGE, w1);
+            if (INT8) read_rows(lds + (uint32_t)after * STAGE, 0, x1);
+            else read_rows(lds + (uint32_t)after * STAGE, 0, x);
+        }
+        if (INT8) {
+            multiply_i8(w, x);
+            x = x1;
+        } else
+            multiply_f16(w, x1, 1);
+        w = w1;
+        stage = after;
     }
     // the halves' sums: those of the second through LDS to the waves of the first
     __syncthreads();
@@ -499,18 +540,14 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
     __syncthreads();
     if (half) return;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < MT; ++u) acc[t][u] += other[(t * MT + u) * 64];
-#pragma unroll
     for (int u = 0; u < MT; ++u) {
-        const int m = blockIdx.y * BLOCK_ROWS + (u0 + u) * 16 + col;
+        const int m = blockIdx.y * BLOCK_ROWS + u * 16 + col;
         if (m >= a.M) continue;
         const float f = INT8 ? a.x_scale[m] * 0.0625f : back[m];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int n = (t0 + n_wave + t) * 16 + 4 * q;
-            f4 y = acc[t][u] * f;
+            f4 y = (acc[t][u] + other[(t * MT + u) * 64]) * f;
             float *const to = a.y + (uint64_t)m * a.N + n;
             if (n + 4 <= a.N) {
                 if (a.bias) y += *reinterpret_cast<const f4u *>(a.bias + n);
