@@ -28,7 +28,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 // bits of the float16 1024 + c + 8, or, four places up, of 64 + c + 8; taking 1032 or 72 off is exact.
 __device__ __forceinline__ h8 weights_f16(uint32_t w) {
     uint32_t low = 0x000f000fu, high = 0x00f000f0u, at10 = 0x64006400u, at6 = 0x54005400u;
-    asm("" : "+s"(low), "+s"(high), "+s"(at10), "+s"(at6));      // registers: one instruction takes no two constants of 32 bits
+    asm("" : "+s"(low), "+s"(high), "+v"(at10), "+v"(at6));      // registers: an instruction takes one constant or scalar
     const uint32_t u = w ^ 0x88888888u, v = u >> 8;
     const h2 far = {(_Float16)1032.f, (_Float16)1032.f}, near = {(_Float16)72.f, (_Float16)72.f};
     const h2 a = __builtin_bit_cast(h2, (u & low) | at10) - far;
@@ -333,8 +333,9 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
 // One workgroup a row.  Rows behind the last one are not written: a column's sums are its own.
 constexpr int BLOCK_ROWS = 64;
 constexpr uint32_t piece_bytes(bool int8) { return int8 ? 64 * 128 : 64 * 128 * 4; }
-constexpr int many_stages(bool int8) { return int8 ? 5 : 3; }
-constexpr uint32_t many_lds_bytes(bool int8) { return many_stages(int8) * (piece_bytes(int8) + 9 * 1024); }
+constexpr int many_stages(bool int8) { return int8 ? 4 : 2; }
+constexpr uint32_t many_stage_bytes(bool int8) { return 2 * piece_bytes(int8) + (int8 ? 2 * (8 + 1) * 1024 : 0); }       // rows of two chunks; their codes and scales
+constexpr uint32_t many_lds_bytes(bool int8) { return many_stages(int8) * many_stage_bytes(int8); }
 
 template <bool INT8>
 __global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, char *operand, float *back) {
@@ -379,51 +380,64 @@ __global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, char *operand
     }
 }
 
-// A workgroup of eight waves has 128 outputs and 64 rows, a wave 32 of the outputs, all the rows and one half of each chunk's
-// inputs.  Rows, codes and scales of a chunk are loaded straight into one of a ring of stages in LDS, STAGES - 1 chunks
-// ahead of the one that is multiplied, and a step's operands are read from there while the step before it is multiplied: one workgroup a
-// compute unit has nobody else to hide a wait behind.  Each weight is turned into float16 by one wave only, for 64 rows: that takes
-// the vector unit as long as the multiplications take the matrix unit where two waves do it for 32 rows each.
+// A workgroup of eight waves has 128 outputs and 64 rows, a wave 32 of the outputs, all the rows and every other chunk of
+// inputs.  The rows of two chunks are loaded straight into a stage in LDS while those of another stage are multiplied, and a step's operands
+// are read from there while the step before it is multiplied: one workgroup a compute unit has nobody else to hide a wait behind.
+// Each weight is turned into float16 by one wave only, for 64 rows: where two waves do it for 32 rows each, that takes
+// the vector unit as long as the multiplications take the matrix unit.  float32 rows fill the LDS with two stages, and a wave loads its codes
+// and scales into registers; 8-bit rows, which are multiplied faster than a load comes back, leave room for four stages with
+// codes and scales.
 template <int G, bool INT8>
 __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char *operand, const float *back) {
-    constexpr uint32_t ROWS = piece_bytes(INT8), CODES = 8 * 1024, SCALES = 1024, STAGE = ROWS + CODES + SCALES;
-    constexpr int STAGES = many_stages(INT8), LOADS = ROWS / 8192 + CODES / 8192 + 1;       // of a wave for a chunk
+    constexpr uint32_t ROWS = piece_bytes(INT8), STAGE = many_stage_bytes(INT8);
+    constexpr int STAGES = many_stages(INT8), LOADS = 2 * ROWS / 8192 + (INT8 ? 4 : 0);      // of a wave for a stage, straight into LDS
     constexpr int GROUPS = 128 / G, NT = 2, MT = 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, col = lane & 15;
-    const int tiles = a.cols / 16, t0 = blockIdx.x * 8, n_wave = (wave & 3) * NT, half = wave >> 2;
+    const int tiles = a.cols / 16, t0 = blockIdx.x * 8, n_wave = (wave & 3) * NT, half = wave >> 2, pairs = (a.chunks + 1) / 2;
     const char *const block = operand + (uint64_t)blockIdx.y * a.chunks * ROWS;
+    const uint8_t *const own_codes = a.codes + (uint64_t)min(t0 + wave, tiles - 1) * a.chunks * 1024;
     const uint32_t lds0 = (uint32_t)(uintptr_t)&lds[0];
     // scales: 16 lanes for the 256 bytes of a group's 128 outputs; what lies behind the row of scales reads as zero
-    const uint32_t row_bytes = (uint32_t)min(256, (a.cols - t0 * 16) * 2);
-    auto issue = [&](int c, int at_stage) {
+    const uint32_t row_bytes = (uint32_t)min(256, (a.cols - t0 * 16) * 2), in_row = (uint32_t)col * 16;
+    auto issue = [&](int p, int at_stage) {          // what lies behind the last chunk reads as zero
         const uint32_t to = lds0 + (uint32_t)at_stage * STAGE;
-        const xsmi::xsmi_int32x4 rows = xsmi::make_rsrc(block + (uint64_t)c * ROWS, ROWS);
+        const int left = min(2, a.chunks - 2 * p);
+        const xsmi::xsmi_int32x4 rows = xsmi::make_rsrc(block + (uint64_t)(2 * p) * ROWS, (uint32_t)left * ROWS);
 #pragma unroll
-        for (uint32_t i = 0; i < ROWS / 8192; ++i) {
-            const uint32_t at = (i * 8 + wave) * 1024;
-            xsmi::load_lds_b128(rows, to + at, at + lane * 16, 0);
+        for (uint32_t i = 0; i < 2 * ROWS / 8192; ++i) xsmi::load_lds_b128(rows, to + (i * 8 + wave) * 1024, lane * 16, (i * 8 + wave) * 1024);
+        if (INT8) {
+            const xsmi::xsmi_int32x4 codes = xsmi::make_rsrc(own_codes + (uint64_t)(2 * p) * 1024, (uint32_t)left * 1024);
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                xsmi::load_lds_b128(codes, to + 2 * ROWS + (i * 8 + wave) * 1024, lane * 16, i * 1024);
+                // group (lane >> 4) of the chunk; the same by every wave, so that all have as many loads under way
+                const xsmi::xsmi_int32x4 scales = xsmi::make_rsrc(a.scales + (uint64_t)min(2 * p + (int)i, a.chunks - 1) * GROUPS * a.cols + t0 * 16,
+                                                                  (uint32_t)(GROUPS - 1) * a.cols * 2 + row_bytes);
+                xsmi::load_lds_b128(scales, to + 2 * ROWS + 16384 + i * 1024, q < GROUPS && in_row < row_bytes ? (uint32_t)q * a.cols * 2 + in_row : 0x80000000u, 0);
+            }
         }
-        const xsmi::xsmi_int32x4 codes = xsmi::make_rsrc(a.codes + ((uint64_t)min(t0 + wave, tiles - 1) * a.chunks + c) * 1024, 1024);
-        xsmi::load_lds_b128(codes, to + ROWS + wave * 1024, lane * 16, 0);
-        // group (lane >> 4) of the chunk; the same by every wave, so that all have as many loads under way
-        const xsmi::xsmi_int32x4 scales = xsmi::make_rsrc(a.scales + (uint64_t)c * GROUPS * a.cols + t0 * 16, (uint32_t)(GROUPS - 1) * a.cols * 2 + row_bytes);
-        const uint32_t in = (uint32_t)(lane & 15) * 16;
-        xsmi::load_lds_b128(scales, to + ROWS + CODES, (lane >> 4) < GROUPS && in < row_bytes ? (uint32_t)(lane >> 4) * a.cols * 2 + in : 0x80000000u, 0);
     };
-    // what a wave multiplies of a chunk: steps 2 half and 2 half + 1 of codes, their scales; rows a step at a time
-    constexpr int OWN = GROUPS == 4 ? 2 : 1;
     struct Weights {
-        u2 w[NT];
-        h4 s[NT][OWN];
+        u4 w[NT];
+        h4 s[NT][GROUPS];
+    };
+    auto load_weights = [&](int p, Weights &r) {
+        const int c = min(2 * p + half, a.chunks - 1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int tile = min(t0 + n_wave + t, tiles - 1);
+            r.w[t] = reinterpret_cast<const u4 *>(a.codes)[((uint64_t)tile * a.chunks + c) * 64 + lane];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) r.s[t][g] = *reinterpret_cast<const h4 *>(a.scales + (uint64_t)(c * GROUPS + g) * a.cols + tile * 16 + 4 * q);
+        }
     };
     auto read_weights = [&](const char *stage, Weights &r) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            r.w[t] = reinterpret_cast<const u2 *>(stage + ROWS)[((n_wave + t) * 64 + lane) * 2 + half];
+            r.w[t] = reinterpret_cast<const u4 *>(stage + 2 * ROWS)[(half * 8 + n_wave + t) * 64 + lane];
 #pragma unroll
-            for (int g = 0; g < OWN; ++g)
-                r.s[t][g] = *reinterpret_cast<const h4 *>(stage + ROWS + CODES + (2 * half + g) / (G / 32) * 256 + (n_wave + t) * 32 + q * 8);
+            for (int g = 0; g < GROUPS; ++g) r.s[t][g] = *reinterpret_cast<const h4 *>(stage + 2 * ROWS + 16384 + half * 1024 + g * 256 + (n_wave + t) * 32 + q * 8);
         }
     };
     struct Rows {
@@ -434,7 +448,7 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
         for (int u = 0; u < MT; ++u)
 #pragma unroll
             for (int p = 0; p < (INT8 ? 1 : 2); ++p)
-                r.x[p][u] = reinterpret_cast<const u4 *>(stage)[INT8 ? (half * 4 + u) * 64 + lane : (((2 * half + step) * 4 + u) * 2 + p) * 64 + lane];
+                r.x[p][u] = reinterpret_cast<const u4 *>(stage + half * ROWS)[((step * 4 + u) * (INT8 ? 1 : 2) + p) * 64 + lane];
     };
     f4 acc[NT][MT];
 #pragma unroll
@@ -442,33 +456,47 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
 #pragma unroll
         for (int u = 0; u < MT; ++u) acc[t][u] = f4{0.f, 0.f, 0.f, 0.f};
     f4 d[NT][MT];
-    auto multiply_f16 = [&](const Weights &r, const Rows &x, int step) {
-        h8 w[NT];
+    // One step's multiplications, with the next step's weights and rows made ready between them: a multiplication takes the matrix unit
+    // four times as long as it takes to issue, and the two waves of a SIMD go through their steps together.
+    auto multiply_f16 = [&](const Weights &r, const h8 *w, const Rows &x, int step, h8 *w_next, const char *stage, Rows &x_next) {
+        if (step < 3) read_rows(stage, step + 1, x_next);
+        __builtin_amdgcn_sched_barrier(0);
+        if (step < 3) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) w[t] = weights_f16(step ? r.w[t].y : r.w[t].x);
+            for (int t = 0; t < NT; ++t) w_next[t] = weights_f16(r.w[t][step + 1]);
+        }
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
             for (int u = 0; u < MT; ++u)
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const f4 from = p == 0 && (G == 32 || step == 0) ? f4{0.f, 0.f, 0.f, 0.f} : d[t][u];
+                    const f4 from = p == 0 && step % (G / 32) == 0 ? f4{0.f, 0.f, 0.f, 0.f} : d[t][u];
                     d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[t], __builtin_bit_cast(h8, x.x[INT8 ? 0 : p][u]), from, 0, 0, 0);
                 }
-        if (G == 32 || step == 1) {
+        if (step < 3) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       // multiplication
+                __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);       // vector
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if ((step + 1) % (G / 32) == 0) {
 #pragma unroll
             for (int u = 0; u < MT; ++u)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)r.s[t][step % OWN][v] * d[t][u][v];
+                    for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)r.s[t][step / (G / 32)][v] * d[t][u][v];
         }
     };
-    auto multiply_i8 = [&](const Weights &r, const Rows &x) {
+    i4 n[NT][MT];
+    auto multiply_i8 = [&](const Weights &r, const Rows &x, int step) {      // steps of 64 inputs
         const i4 zero = {0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const u2 lo = weights_i8(r.w[t].x), hi = weights_i8(r.w[t].y);
+            const u2 lo = weights_i8(r.w[t][2 * step]), hi = weights_i8(r.w[t][2 * step + 1]);
 #pragma unroll
             for (int u = 0; u < MT; ++u) {
                 const u4 b = x.x[0][u];
@@ -477,56 +505,54 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
                     const i4 f = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, hi), __builtin_bit_cast(long, u2{b.z, b.w}), zero, 0, 0, 0);
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
-                        acc[t][u][v] += (float)r.s[t][0][v] * (float)e[v];
-                        acc[t][u][v] += (float)r.s[t][OWN - 1][v] * (float)f[v];
+                        acc[t][u][v] += (float)r.s[t][2 * step % GROUPS][v] * (float)e[v];
+                        acc[t][u][v] += (float)r.s[t][(2 * step + 1) % GROUPS][v] * (float)f[v];
                     }
                 } else {
-                    const i4 e = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y}, __builtin_bit_cast(i4, b), zero, 0, 0, 0);
+                    n[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y}, __builtin_bit_cast(i4, b),
+                                                                    G == 64 || step == 0 ? zero : n[t][u], 0, 0, 0);
+                    if (G == 64 || step == 1) {
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)r.s[t][0][v] * (float)e[v];
+                        for (int v = 0; v < 4; ++v) acc[t][u][v] += (float)r.s[t][step % GROUPS][v] * (float)n[t][u][v];
+                    }
                 }
             }
         }
     };
-    // A chunk can be read once this wave's loads of it have arrived (no more than the later chunks' are under way) and, behind
-    // the barrier, everybody's have; the chunk before it has been read by then: its stage is loaded anew after that.
-    auto arrive = [&](int c) {
-        if (c + STAGES - 1 <= a.chunks) xsmi::wait_vmcnt<LOADS * (STAGES - 2)>(); else xsmi::wait_vmcnt<0>();
-        xsmi::wait_lgkmcnt0();
-        xsmi::block_barrier();
-    };
+    Weights w, next;
 #pragma unroll
-    for (int c = 0; c < STAGES - 1; ++c)
-        if (c < a.chunks) issue(c, c);
-    Weights w;
-    Rows x;
-    arrive(0);
-    read_weights(lds, w);
-    read_rows(lds, 0, x);
+    for (int p = 0; p < STAGES - 1; ++p)
+        if (p < pairs) issue(p, p);
+    if (!INT8) load_weights(0, w);
     int stage = 0;
-    for (int c = 0; c < a.chunks; ++c) {
-        const int after = stage + 1 == STAGES ? 0 : stage + 1;
-        const bool more = c + 1 < a.chunks;
-        if (c + STAGES - 1 < a.chunks) issue(c + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);      // where chunk c - 1 was
-        Weights w1;
-        Rows x1;
-        if (!INT8) {
-            read_rows(lds + (uint32_t)stage * STAGE, 1, x1);
-            multiply_f16(w, x, 0);
+    for (int p = 0; p < pairs; ++p) {
+        // This wave's loads of the stage have arrived (no more than the later stages' are under way) and, behind the barrier,
+        // everybody's have; and everybody has read the stage before it, which is loaded anew.
+        if (INT8 && p + STAGES - 1 <= pairs) xsmi::wait_vmcnt<LOADS *(STAGES - 2)>(); else xsmi::wait_vmcnt<0>();
+        xsmi::block_barrier();
+        if (p + STAGES - 1 < pairs) issue(p + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        const char *const from = lds + (uint32_t)stage * STAGE;
+        Rows x, y;
+        if (INT8) read_weights(from, w); else load_weights(p + 1, next);
+        if (2 * p + half < a.chunks) {
+            read_rows(from, 0, x);
+            if (INT8) {
+                read_rows(from, 1, y);
+                multiply_i8(w, x, 0);
+                multiply_i8(w, y, 1);
+            } else {
+                h8 v0[NT], v1[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) v0[t] = weights_f16(w.w[t][0]);
+                multiply_f16(w, v0, x, 0, v1, from, y);
+                multiply_f16(w, v1, y, 1, v0, from, x);
+                multiply_f16(w, v0, x, 2, v1, from, y);
+                multiply_f16(w, v1, y, 3, v0, from, x);
+            }
         }
-        if (more) {
-            arrive(c + 1);
-            read_weights(lds + (uint32_t)after * STAGE, w1);
-            if (INT8) read_rows(lds + (uint32_t)after * STAGE, 0, x1);
-            else read_rows(lds + (uint32_t)after * STAGE, 0, x);
-        }
-        if (INT8) {
-            multiply_i8(w, x);
-            x = x1;
-        } else
-            multiply_f16(w, x1, 1);
-        w = w1;
-        stage = after;
+        if (!INT8) w = next;
+        xsmi::wait_lgkmcnt0();                       // read, before the barrier that lets the stage go
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     // the halves' sums: those of the second through LDS to the waves of the first
     __syncthreads();
