@@ -31,24 +31,32 @@ __device__ __forceinline__ V row_sum(V v, V *sm) {
     return v;
 }
 
+// The sum of one value and the largest of another, likewise.
 template <int T>
-__device__ __forceinline__ double row_max(double v, double *sm) {
+__device__ __forceinline__ void row_sum_max(double &sum, double &most, double2 *sm) {
 #pragma unroll
-    for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
+    for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) {
+        sum += __shfl_xor(sum, o);
+        most = fmax(most, __shfl_xor(most, o));
+    }
     if (T > 64) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = make_double2(sum, most);
         __syncthreads();
         const int first = threadIdx.x / T * (T / 64);
-        v = sm[first];
+        sum = sm[first].x;
+        most = sm[first].y;
 #pragma unroll
-        for (int w = 1; w < T / 64; ++w) v = fmax(v, sm[first + w]);
+        for (int w = 1; w < T / 64; ++w) {
+            sum += sm[first + w].x;
+            most = fmax(most, sm[first + w].y);
+        }
     }
-    return v;
 }
 
+// STREAM: past the caches' replacement, for operands that are larger than they are.
+template <bool STREAM = false>
 __device__ __forceinline__ f4 load4(const float *p, int j, int cols) {
-    if (j + 4 <= cols) return *reinterpret_cast<const f4u *>(p + j);
+    if (j + 4 <= cols) return STREAM ? __builtin_nontemporal_load(reinterpret_cast<const f4u *>(p + j)) : *reinterpret_cast<const f4u *>(p + j);
     f4 r = {0.f, 0.f, 0.f, 0.f};
     if (j < cols) r.x = p[j];
     if (j + 1 < cols) r.y = p[j + 1];
@@ -56,9 +64,11 @@ __device__ __forceinline__ f4 load4(const float *p, int j, int cols) {
     return r;
 }
 
+template <bool STREAM = false>
 __device__ __forceinline__ void store4(float *p, int j, int cols, f4 v) {
     if (j + 4 <= cols) {
-        *reinterpret_cast<f4u *>(p + j) = v;
+        if (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<f4u *>(p + j));
+        else *reinterpret_cast<f4u *>(p + j) = v;
         return;
     }
     if (j < cols) p[j] = v.x;
@@ -77,7 +87,7 @@ struct Forward {
 };
 
 // T threads a row, NT threads a workgroup, V vectors of four a thread: rows of up to 4 T V elements stay in registers.
-template <int T, int NT, int V>
+template <int T, int NT, int V, bool STREAM>
 __global__ void __launch_bounds__(NT) rms_fwd_kernel(Forward a) {
     __shared__ float sm[NT / 64];
     const uint64_t row = (uint64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
@@ -91,8 +101,8 @@ __global__ void __launch_bounds__(NT) rms_fwd_kernel(Forward a) {
         const int j = 4 * (v * T + t);
         s[v] = f4{0.f, 0.f, 0.f, 0.f};
         if (live && j < cols) {
-            s[v] = load4(a.x + at, j, cols);
-            if (a.residual) s[v] += load4(a.residual + at, j, cols);
+            s[v] = load4<STREAM>(a.x + at, j, cols);
+            if (a.residual) s[v] += load4<STREAM>(a.residual + at, j, cols);
         }
     }
 #pragma unroll
@@ -107,8 +117,8 @@ __global__ void __launch_bounds__(NT) rms_fwd_kernel(Forward a) {
     for (int v = 0; v < V; ++v) {
         const int j = 4 * (v * T + t);
         if (j < cols) {
-            if (a.sum) store4(a.sum + at, j, cols, s[v]);
-            store4(a.y + at, j, cols, s[v] * r * load4(a.gamma, j, cols));
+            if (a.sum) store4<STREAM>(a.sum + at, j, cols, s[v]);
+            store4<STREAM>(a.y + at, j, cols, s[v] * r * load4(a.gamma, j, cols));
         }
     }
 }
@@ -149,109 +159,100 @@ __device__ __forceinline__ void store_q(int8_t *p, int j, int cols, const double
         if (j + e < cols) p[j + e] = (int8_t)q[e];
 }
 
-// The output in 8 bits: q_j = round(127 y_j / max |y|), scale = max |y| / 127.  In 64 bits, which run at the rate of 32 here and
+// The output in 8 bits: q_j = round(127 y_j / max |y|), scale = max |y| / 127.  The root is common to a row's y, so the numbers are those of
+// z_j = gamma_j s_j, and the sum and the largest value are found together.  In 64 bits, which run at the rate of 32 here and
 // are not what bounds this: a number next to a border falls on the side that the exact value is on, whatever the order
-// of the sums.
+// of the sums.  A row of zeros has the numbers 0 and the scale 0, one with a NaN or an infinity the numbers 0 and the scale NaN.
+struct Steps {
+    bool bad;
+    double inverse;
+};
+__device__ __forceinline__ Steps steps_of(const Forward &a, double sq, double most, uint64_t row, bool writes) {
+    const bool bad = !(most < INFINITY);
+    if (writes) a.scale[row] = bad ? NAN : most == 0.0 ? 0.f : (float)(most / sqrt(sq / (double)a.cols + (double)a.eps) / 127.0);
+    return Steps{bad, bad || most == 0.0 ? 0.0 : 127.0 / most};
+}
+
 template <int T, int NT, int V>
 __global__ void __launch_bounds__(NT) rms_fwd_int8_kernel(Forward a) {
-    __shared__ double sm[NT / 64];
+    __shared__ double2 sm[NT / 64];
     const uint64_t row = (uint64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
     const int t = threadIdx.x % T, cols = a.cols;
     const bool live = row < a.rows;
     const uint64_t at = row * (uint64_t)cols;
-    f4 s[V];
-    double sq = 0.0;
+    f4 s[V], g[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int j = 4 * (v * T + t);
-        s[v] = f4{0.f, 0.f, 0.f, 0.f};
+        s[v] = g[v] = f4{0.f, 0.f, 0.f, 0.f};
         if (live && j < cols) {
             s[v] = load4(a.x + at, j, cols);
-            if (a.residual) {
-                s[v] += load4(a.residual + at, j, cols);
-                store4(a.sum + at, j, cols, s[v]);
-            }
+            g[v] = load4(a.gamma, j, cols);
+            if (a.residual) s[v] += load4(a.residual + at, j, cols);
         }
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sq += (double)s[v][e] * (double)s[v][e];
-    sq = row_sum<T>(sq, sm);
-    const double r = 1.0 / sqrt(sq / (double)cols + (double)a.eps);
-    double most = 0.0;
+    double sq = 0.0, most = 0.0;
     bool nan = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int j = 4 * (v * T + t);
-        if (live && j < cols) {
-            const f4 g = load4(a.gamma, j, cols);
+        if (a.sum && live && j < cols) store4(a.sum + at, j, cols, s[v]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double y = (double)s[v][e] * r * (double)g[e];
-                nan |= y != y;
-                most = fmax(most, fabs(y));
-            }
+        for (int e = 0; e < 4; ++e) {
+            const double z = (double)s[v][e] * (double)g[v][e];
+            sq += (double)s[v][e] * (double)s[v][e];
+            nan |= z != z;
+            most = fmax(most, fabs(z));
         }
     }
-    most = row_max<T>(nan ? INFINITY : most, sm);
+    most = nan ? INFINITY : most;
+    row_sum_max<T>(sq, most, sm);
     if (!live) return;
-    // A row of zeros has the numbers 0 and the scale 0; one with a NaN or an infinity the numbers 0 and the scale NaN.
-    const bool bad = !(most < INFINITY);
-    const double inverse = bad || most == 0.0 ? 0.0 : 127.0 / most;
-    if (t == 0) a.scale[row] = bad ? NAN : (float)(most / 127.0);
+    const Steps step = steps_of(a, sq, most, row, t == 0);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int j = 4 * (v * T + t);
         if (j < cols) {
-            const f4 g = load4(a.gamma, j, cols);
-            double y[4];
+            double z[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = bad ? 0.0 : (double)s[v][e] * r * (double)g[e];
-            store_q(a.q + at, j, cols, y, inverse);
+            for (int e = 0; e < 4; ++e) z[e] = step.bad ? 0.0 : (double)s[v][e] * (double)g[v][e];
+            store_q(a.q + at, j, cols, z, step.inverse);
         }
     }
 }
 
 template <int NT>
 __global__ void __launch_bounds__(NT) rms_fwd_int8_long_kernel(Forward a) {
-    __shared__ double sm[NT / 64];
+    __shared__ double2 sm[NT / 64];
     const uint64_t row = blockIdx.x, at = row * (uint64_t)a.cols;
     const int cols = a.cols;
-    double sq = 0.0;
+    double sq = 0.0, most = 0.0;
+    bool nan = false;
     for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
         f4 s = load4(a.x + at, j, cols);
+        const f4 g = load4(a.gamma, j, cols);
         if (a.residual) {
             s += load4(a.residual + at, j, cols);
             store4(a.sum + at, j, cols, s);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sq += (double)s[e] * (double)s[e];
-    }
-    sq = row_sum<NT>(sq, sm);
-    const double r = 1.0 / sqrt(sq / (double)cols + (double)a.eps);
-    const float *from = a.residual ? a.sum + at : a.x + at;
-    double most = 0.0;
-    bool nan = false;
-    for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
-        const f4 s = load4(from, j, cols), g = load4(a.gamma, j, cols);
-#pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const double y = (double)s[e] * r * (double)g[e];
-            nan |= y != y;
-            most = fmax(most, fabs(y));
+            const double z = (double)s[e] * (double)g[e];
+            sq += (double)s[e] * (double)s[e];
+            nan |= z != z;
+            most = fmax(most, fabs(z));
         }
     }
-    most = row_max<NT>(nan ? INFINITY : most, sm);
-    const bool bad = !(most < INFINITY);
-    const double inverse = bad || most == 0.0 ? 0.0 : 127.0 / most;
-    if (threadIdx.x == 0) a.scale[row] = bad ? NAN : (float)(most / 127.0);
+    most = nan ? INFINITY : most;
+    row_sum_max<NT>(sq, most, sm);
+    const Steps step = steps_of(a, sq, most, row, threadIdx.x == 0);
+    const float *from = a.residual ? a.sum + at : a.x + at;
     for (int j = 4 * threadIdx.x; j < cols; j += 4 * NT) {
         const f4 s = load4(from, j, cols), g = load4(a.gamma, j, cols);
-        double y[4];
+        double z[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = bad ? 0.0 : (double)s[e] * r * (double)g[e];
-        store_q(a.q + at, j, cols, y, inverse);
+        for (int e = 0; e < 4; ++e) z[e] = step.bad ? 0.0 : (double)s[e] * (double)g[e];
+        store_q(a.q + at, j, cols, z, step.inverse);
     }
 }
 
@@ -264,8 +265,9 @@ struct Backward {
 };
 
 // T threads a row; a workgroup takes every (NT / T gridDim)-th lot of rows, and adds the terms of dgamma of the columns
-// that a thread owns in its registers; they go to part[group of rows] at the end.
-template <int T, int NT, int V>
+// that a thread owns in its registers; they go to part[group of rows] at the end.  All that a row needs is loaded before its sum is
+// formed.
+template <int T, int NT, int V, bool STREAM>
 __global__ void __launch_bounds__(NT) rms_bwd_kernel(Backward a) {
     __shared__ float sm[NT / 64];
     const int t = threadIdx.x % T, cols = a.cols;
@@ -280,16 +282,17 @@ __global__ void __launch_bounds__(NT) rms_bwd_kernel(Backward a) {
     for (uint64_t first = (uint64_t)blockIdx.x * (NT / T); first < a.rows; first += (uint64_t)gridDim.x * (NT / T)) {
         const uint64_t row = first + threadIdx.x / T, at = row * (uint64_t)cols;
         const bool live = row < a.rows;
-        f4 s[V], d[V];
+        f4 s[V], d[V], g[V];
         float c = 0.f;
         const float r = live ? a.rstd[row] : 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int j = 4 * (v * T + t);
-            s[v] = d[v] = f4{0.f, 0.f, 0.f, 0.f};
+            s[v] = d[v] = g[v] = f4{0.f, 0.f, 0.f, 0.f};
             if (live && j < cols) {
-                s[v] = load4(a.s + at, j, cols);
-                d[v] = load4(a.dy + at, j, cols);
+                s[v] = load4<STREAM>(a.s + at, j, cols);
+                d[v] = load4<STREAM>(a.dy + at, j, cols);
+                if (a.ds) g[v] = load4<STREAM>(a.ds + at, j, cols);
             }
         }
 #pragma unroll
@@ -306,16 +309,9 @@ __global__ void __launch_bounds__(NT) rms_bwd_kernel(Backward a) {
             for (int v = 0; v < V; ++v) {
                 const int j = 4 * (v * T + t);
                 if (j < cols) {
-                    f4 g = (d[v] - s[v] * c) * r;
-                    if (a.ds) g += load4(a.ds + at, j, cols);
-                    f4 o = g;
-                    if (a.acc1) o += load4(a.dx1 + at, j, cols);
-                    store4(a.dx1 + at, j, cols, o);
-                    if (a.dx2) {
-                        o = g;
-                        if (a.acc2) o += load4(a.dx2 + at, j, cols);
-                        store4(a.dx2 + at, j, cols, o);
-                    }
+                    g[v] += (d[v] - s[v] * c) * r;
+                    store4<STREAM>(a.dx1 + at, j, cols, a.acc1 ? g[v] + load4(a.dx1 + at, j, cols) : g[v]);
+                    if (a.dx2) store4<STREAM>(a.dx2 + at, j, cols, a.acc2 ? g[v] + load4(a.dx2 + at, j, cols) : g[v]);
                 }
             }
         }
@@ -358,19 +354,28 @@ __global__ void __launch_bounds__(NT) rms_bwd_long_kernel(Backward a) {
     }
 }
 
-// dgamma[j] = (accumulate ? dgamma[j] : 0) + sum over the rows of part: 64 columns and 16 stretches of rows a workgroup.
+// dgamma[j] = (accumulate ? dgamma[j] : 0) + sum over the rows of part: 32 columns a workgroup, eight threads of four columns for each
+// of 128 stretches of rows.
 __global__ void __launch_bounds__(1024) rms_dgamma_kernel(const float *__restrict__ part, int rows, int cols, float *dgamma, int accumulate) {
-    __shared__ float sm[16][64];
-    const int j = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-    float s = 0.f;
-    if (j < cols)
-        for (int i = w; i < rows; i += 16) s += part[(uint64_t)i * cols + j];
-    sm[w][threadIdx.x & 63] = s;
+    __shared__ f4 sm[128][8];
+    const int t = threadIdx.x & 7, j = blockIdx.x * 32 + 4 * t, w = threadIdx.x >> 3;
+    f4 s = {0.f, 0.f, 0.f, 0.f};
+    if (j < cols) {
+#pragma unroll 4
+        for (int i = w; i < rows; i += 128) s += load4(part + (uint64_t)i * cols, j, cols);
+    }
+    sm[w][t] = s;
     __syncthreads();
+    for (int n = 64; n >= 8; n >>= 1) {              // the stretches by halves, the last eight one after the other
+        if (w < n) sm[w][t] += sm[w + n][t];
+        __syncthreads();
+    }
     if (w == 0 && j < cols) {
-        float r = 0.f;
-        for (int i = 0; i < 16; ++i) r += sm[i][threadIdx.x];
-        dgamma[j] = accumulate ? dgamma[j] + r : r;
+        f4 r = sm[0][t];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) r += sm[i][t];
+        if (accumulate) r += load4(dgamma, j, cols);
+        store4(dgamma, j, cols, r);
     }
 }
 
@@ -383,11 +388,12 @@ struct BackwardPlan {
 BackwardPlan backward_plan(uint64_t rows, int cols) {
     BackwardPlan p;
     const int need = (cols + 3) / 4;
-    p.threads_a_row = need <= 16 ? 16 : need <= 64 ? 64 : need <= 1024 ? 256 : 1024;
+    p.threads_a_row = need <= 16 ? 16 : need <= 64 ? 64 : need <= 256 ? 256 : 1024;
     p.threads = p.threads_a_row == 1024 ? 1024 : 256;
     const uint64_t lots = (rows + p.threads / p.threads_a_row - 1) / (p.threads / p.threads_a_row);
-    const uint64_t most = p.threads == 1024 ? 256 : 1024;
-    p.groups = (int)(lots < most ? lots : most);
+    // as many workgroups as fill the card, and at least two lots of rows each where there are more than two a compute unit
+    const uint64_t most = need > 1024 ? 256 : 1024, few = most / 2, two = (lots + 1) / 2;
+    p.groups = (int)(lots <= few ? lots : two <= few ? few : two < most ? two : most);
     p.parts = p.groups * (p.threads / p.threads_a_row);
     return p;
 }
@@ -399,7 +405,17 @@ int check(const char *who, size_t rows, int cols, float eps) {
     return XSMI_OK;
 }
 
+// Operands past the last-level cache (256 MB) are streamed: 16384 rows of 4096, backward 252 us without, 226 with; where they
+// fit, the next kernel finds them there.
+inline bool streams(size_t rows, int cols, int operands) { return (double)rows * cols * operands * 4 > 256e6; }
+
 #define LAUNCH(kernel, grid, threads, args) hipLaunchKernelGGL(kernel, dim3((uint32_t)(grid)), dim3(threads), 0, xsmi::stream(), args)
+
+#define LAUNCH_TWO(kernel, T, NT, V, grid, args)                          \
+    do {                                                                 \
+        if (stream) LAUNCH((kernel<T, NT, V, true>), grid, NT, args);    \
+        else LAUNCH((kernel<T, NT, V, false>), grid, NT, args);          \
+    } while (0)
 
 }  // namespace
 
@@ -412,12 +428,13 @@ int xsmi_rms_norm_fwd(const float *x, const float *residual, const float *gamma,
     if (rows == 0) return XSMI_OK;
     XSMI_CHECK_ARG(x && gamma && y && (residual == nullptr) == (sum == nullptr), "xsmi_rms_norm_fwd: null pointer (a residual comes with a sum)");
     const Forward a = {x, residual, gamma, sum, y, rstd, nullptr, nullptr, rows, cols, eps};
+    const bool stream = streams(rows, cols, residual ? 4 : 2);
     const int need = (cols + 3) / 4;
-    if (need <= 16) LAUNCH((rms_fwd_kernel<16, 256, 1>), (rows + 15) / 16, 256, a);
-    else if (need <= 64) LAUNCH((rms_fwd_kernel<64, 256, 1>), (rows + 3) / 4, 256, a);
-    else if (need <= 256) LAUNCH((rms_fwd_kernel<256, 256, 1>), rows, 256, a);
-    else if (need <= 1024) LAUNCH((rms_fwd_kernel<256, 256, 4>), rows, 256, a);
-    else if (need <= 4096) LAUNCH((rms_fwd_kernel<1024, 1024, 4>), rows, 1024, a);
+    if (need <= 16) LAUNCH_TWO(rms_fwd_kernel, 16, 256, 1, (rows + 15) / 16, a);
+    else if (need <= 64) LAUNCH_TWO(rms_fwd_kernel, 64, 256, 1, (rows + 3) / 4, a);
+    else if (need <= 256) LAUNCH_TWO(rms_fwd_kernel, 256, 256, 1, rows, a);
+    else if (need <= 1024) LAUNCH_TWO(rms_fwd_kernel, 512, 512, 2, rows, a);
+    else if (need <= 4096) LAUNCH_TWO(rms_fwd_kernel, 1024, 1024, 4, rows, a);
     else LAUNCH((rms_fwd_long_kernel<1024>), rows, 1024, a);
     XSMI_LAUNCH_CHECK("rms_fwd_kernel");
     return XSMI_OK;
@@ -434,7 +451,7 @@ int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma
     if (need <= 16) LAUNCH((rms_fwd_int8_kernel<16, 256, 1>), (rows + 15) / 16, 256, a);
     else if (need <= 64) LAUNCH((rms_fwd_int8_kernel<64, 256, 1>), (rows + 3) / 4, 256, a);
     else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1>), rows, 256, a);
-    else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<256, 256, 4>), rows, 256, a);
+    else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 1>), rows, 1024, a);
     else if (need <= 4096) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 4>), rows, 1024, a);
     else LAUNCH((rms_fwd_int8_long_kernel<1024>), rows, 1024, a);
     XSMI_LAUNCH_CHECK("rms_fwd_int8_kernel");
@@ -460,16 +477,17 @@ int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const 
     if (!dx1 && !dgamma) return XSMI_OK;
     const BackwardPlan p = backward_plan(rows, cols);
     const Backward a = {dy, s, rstd, gamma, ds, dx1, dx2, dgamma ? (float *)ws : nullptr, beta1 != 0.f, beta2 != 0.f, rows, cols};
+    const bool stream = streams(rows, cols, 3 + (ds != nullptr) + (dx2 != nullptr));
     const int need = (cols + 3) / 4;
-    if (need <= 16) LAUNCH((rms_bwd_kernel<16, 256, 1>), p.groups, 256, a);
-    else if (need <= 64) LAUNCH((rms_bwd_kernel<64, 256, 1>), p.groups, 256, a);
-    else if (need <= 256) LAUNCH((rms_bwd_kernel<256, 256, 1>), p.groups, 256, a);
-    else if (need <= 1024) LAUNCH((rms_bwd_kernel<256, 256, 4>), p.groups, 256, a);
-    else if (need <= 4096) LAUNCH((rms_bwd_kernel<1024, 1024, 4>), p.groups, 1024, a);
+    if (need <= 16) LAUNCH_TWO(rms_bwd_kernel, 16, 256, 1, p.groups, a);
+    else if (need <= 64) LAUNCH_TWO(rms_bwd_kernel, 64, 256, 1, p.groups, a);
+    else if (need <= 256) LAUNCH_TWO(rms_bwd_kernel, 256, 256, 1, p.groups, a);
+    else if (need <= 1024) LAUNCH_TWO(rms_bwd_kernel, 1024, 1024, 1, p.groups, a);
+    else if (need <= 4096) LAUNCH_TWO(rms_bwd_kernel, 1024, 1024, 4, p.groups, a);
     else LAUNCH((rms_bwd_long_kernel<1024>), p.groups, 1024, a);
     XSMI_LAUNCH_CHECK("rms_bwd_kernel");
     if (dgamma) {
-        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((cols + 63) / 64), dim3(1024), 0, xsmi::stream(), (const float *)ws, p.parts, cols, dgamma,
+        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((cols + 31) / 32), dim3(1024), 0, xsmi::stream(), (const float *)ws, p.parts, cols, dgamma,
                            beta_gamma != 0.f);
         XSMI_LAUNCH_CHECK("rms_dgamma_kernel");
     }
