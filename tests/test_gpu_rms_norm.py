@@ -279,7 +279,7 @@ def test_refusals():
     raw = lambda *a: be.lib.call("xsmi_rms_norm_bwd", *a)  # noqa: E731
     p = x.ptr
     for bad in ((p, p, p, p, None, p, 0.5, None, 0.0, None, 0.0, 4, 8, None, 0), (p, p, p, p, None, None, 0.0, p, 0.0, None, 0.0, 4, 8, None, 0),
-                (p, p, p, p, None, p, 0.0, p, 0.0, None, 0.0, 4, 8, None, 0), (p, p, p, p, None, p, 0.0, None, 0.0, p, 0.0, 4, 8, p, 16),
+                (p, p, p, p, None, p, 0.0, p, 0.0, None, 0.0, 4, 8, None, 0), (p, p, p, p, None, p, 0.0, None, 0.0, p, 0.0, 4096, 256, p, 16),
                 (p, p, p, p, None, p, 0.0, None, 0.0, None, 0.0, 4, 0, None, 0), (p, None, p, p, None, p, 0.0, None, 0.0, None, 0.0, 4, 8, None, 0)):
         with pytest.raises(ValueError):
             raw(*bad)

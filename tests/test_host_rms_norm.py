@@ -111,4 +111,4 @@ def test_refusals():
         F.rms_norm_8bit(x, gamma)
     query = capi.lib.raw("xsmi_rms_norm_workspace_bytes")
     assert query(0, 5) == 0 and query(1 << 31, 5) == 0 and query(5, 0) == 0 and query(5, -1) == 0
-    assert query(3, 100) >= 400 and query(1 << 20, 16384) <= 1 << 28
+    assert query(3, 100) == 0 and query(4096, 4096) >= 4 * 4096 and query(1 << 20, 16384) <= 1 << 28

@@ -389,6 +389,16 @@ def empty(shape, dtype=np.float32):
     return DeviceArray(shape, dtype)
 
 
+def empty_like(a):
+    """An array of ``a``'s shape and type, without going over them again."""
+    b = DeviceArray.__new__(DeviceArray)
+    b.shape, b.dtype, b.size, b.nbytes = a.shape, a.dtype, a.size, a.nbytes
+    b._block = _Block(a.nbytes if a.nbytes > 16 else 16)
+    b._block.logical = a.nbytes
+    b._offset = 0
+    return b
+
+
 def zeros(shape, dtype=np.float32, lazy=False):
     return DeviceArray(shape, dtype).fill_zero(lazy)
 

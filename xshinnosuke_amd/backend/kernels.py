@@ -849,41 +849,48 @@ def full(shape, value):
 
 
 # ---- root-mean-square normalisation -----------------------------------------------------------------------------
+_F32, _I8 = np.dtype(np.float32), np.dtype(np.int8)
+
+
 def _rms_operands(x, gamma, residual):
-    if x.dtype != np.float32 or gamma.dtype != np.float32 or (residual is not None and residual.dtype != np.float32):
+    shape = x.shape
+    if x.dtype != _F32 or gamma.dtype != _F32 or (residual is not None and residual.dtype != _F32):
         raise ValueError("rms_norm: operands must be float32")
-    if not x.shape or gamma.size != x.shape[-1]:
-        raise ValueError("rms_norm: %d scales for rows of shape %s" % (gamma.size, x.shape))
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError("rms_norm: residual %s and input %s differ" % (residual.shape, x.shape))
-    cols = x.shape[-1]
-    return (x.size // cols if cols else 0), cols
+    if not shape or shape[-1] == 0 or gamma.size != shape[-1]:
+        raise ValueError("rms_norm: %d scales for rows of shape %s" % (gamma.size, shape))
+    if residual is not None and residual.shape != shape:
+        raise ValueError("rms_norm: residual %s and input %s differ" % (residual.shape, shape))
+    return x.size // shape[-1], shape[-1]
 
 
 def rms_norm_fwd(x, gamma, eps, residual=None, y=None, want_rstd=True):
     """(y, s, rstd): y = gamma * s * rstd over rows of the last axis, s = x + residual (x itself without one),
     rstd = 1 / sqrt(mean(s^2) + eps)."""
     rows, cols = _rms_operands(x, gamma, residual)
-    y = _like(x, y)
-    if cols == 0:
-        raise ValueError("rms_norm: rows without elements")
-    y.take_fresh()
-    s = empty(x.shape) if residual is not None else x
+    if y is None:
+        y = _array.empty_like(x)
+    else:
+        _like(x, y).take_fresh()
     rstd = empty((rows,)) if want_rstd else None
-    lib.call("xsmi_rms_norm_fwd", x.read_ptr, residual.read_ptr if residual is not None else None, gamma.read_ptr,
-             s.ptr if residual is not None else None, y.ptr, rstd.ptr if want_rstd else None, rows, cols, eps)
+    if residual is None:
+        s, summed, other = x, None, None
+    else:
+        s, other = _array.empty_like(x), residual.read_ptr
+        summed = s.ptr
+    lib.call("xsmi_rms_norm_fwd", x.read_ptr, other, gamma.read_ptr, summed, y.ptr, rstd.ptr if want_rstd else None, rows, cols, eps)
     return y, s, rstd
 
 
 def rms_norm_int8(x, gamma, eps, residual=None):
     """(q, scale, s): the same rows as int8 numbers and a float32 scale each."""
     rows, cols = _rms_operands(x, gamma, residual)
-    if cols == 0:
-        raise ValueError("rms_norm: rows without elements")
-    s = empty(x.shape) if residual is not None else x
-    q, scale = empty(x.shape, np.int8), empty(x.shape[:-1])
-    lib.call("xsmi_rms_norm_int8", x.read_ptr, residual.read_ptr if residual is not None else None, gamma.read_ptr,
-             s.ptr if residual is not None else None, q.ptr, scale.ptr, rows, cols, eps)
+    if residual is None:
+        s, summed, other = x, None, None
+    else:
+        s, other = _array.empty_like(x), residual.read_ptr
+        summed = s.ptr
+    q, scale = DeviceArray(x.shape, _I8), empty(x.shape[:-1])
+    lib.call("xsmi_rms_norm_int8", x.read_ptr, other, gamma.read_ptr, summed, q.ptr, scale.ptr, rows, cols, eps)
     return q, scale, s
 
 
@@ -892,21 +899,30 @@ def rms_norm_bwd(dy, s, rstd, gamma, ds=None, dx1=None, dx2=None, dgamma=None):
     each may be None, and one whose clear is pending is overwritten.  dx1 may be ds itself (which then is not added twice)."""
     rows, cols = _rms_operands(s, gamma, None)
     for a in (dy, ds, dx1, dx2):
-        if a is not None and (a.size != s.size or a.dtype != np.float32):
+        if a is not None and (a.size != s.size or a.dtype != _F32):
             raise ValueError("rms_norm_bwd: operand of shape %s for rows of %s" % (a.shape, s.shape))
-    if rstd.size != rows or (dgamma is not None and (dgamma.size != cols or dgamma.dtype != np.float32)):
+    if rstd.size != rows or (dgamma is not None and (dgamma.size != cols or dgamma.dtype != _F32)):
         raise ValueError("rms_norm_bwd: operands do not match %s" % (s.shape,))
-    if ds is not None and ds.is_fresh():
+    if ds is not None and (ds is dx1 or ds.is_fresh()):
         ds = None
-    if ds is not None and ds is dx1:
-        ds = None
-    betas = [0.0 if a is None or a.take_fresh() else 1.0 for a in (dx1, dx2, dgamma)]
-    ws, ws_bytes = None, 0
-    if dgamma is not None and rows:
-        ws, ws_bytes = _ws.get(lib.raw("xsmi_rms_norm_workspace_bytes")(rows, cols))
-    p = [a.ptr if a is not None else None for a in (dx1, dx2, dgamma)]
-    lib.call("xsmi_rms_norm_bwd", dy.read_ptr, s.read_ptr, rstd.read_ptr, gamma.read_ptr, ds.read_ptr if ds is not None else None, p[0], betas[0],
-             p[1], betas[1], p[2], betas[2], rows, cols, ws, ws_bytes)
+    ws, ws_bytes, p1, p2, pg, b1, b2, bg = None, 0, None, None, None, 0.0, 0.0, 0.0
+    if dx1 is not None:
+        b1 = 0.0 if dx1.take_fresh() else 1.0
+        p1 = dx1.ptr
+    if dx2 is not None:
+        b2 = 0.0 if dx2.take_fresh() else 1.0
+        p2 = dx2.ptr
+    if dgamma is not None:
+        bg = 0.0 if dgamma.take_fresh() else 1.0
+        pg = dgamma.ptr
+        key = ("rms", rows, cols)
+        need = _NEED.get(key)
+        if need is None:
+            need = _NEED[key] = lib.raw("xsmi_rms_norm_workspace_bytes")(rows, cols)
+        if need:
+            ws, ws_bytes = _ws.get(need)
+    lib.call("xsmi_rms_norm_bwd", dy.read_ptr, s.read_ptr, rstd.read_ptr, gamma.read_ptr, ds.read_ptr if ds is not None else None, p1, b1,
+             p2, b2, pg, bg, rows, cols, ws, ws_bytes)
 
 
 # ---- dense layers with weights in 4 bits -------------------------------------------------------------------------
@@ -938,20 +954,22 @@ def dequantize_4bit(codes, scales, inputs, outputs, group):
 
 def dense_4bit(x, codes, scales, inputs, outputs, group, bias=None, x_scale=None, out=None):
     """x (rows, inputs) times the packed weight (+ bias over rows): float32 rows, or int8 rows with ``x_scale``."""
-    if x.dtype != (np.float32 if x_scale is None else np.int8):
+    shape = x.shape
+    if x.dtype != (_F32 if x_scale is None else _I8):
         raise ValueError("dense_4bit: rows of %s %s a scale" % (x.dtype, "without" if x_scale is None else "with"))
-    if not x.shape or x.shape[-1] != inputs:
-        raise ValueError("dense_4bit: rows of shape %s for %d inputs" % (x.shape, inputs))
+    if not shape or shape[-1] != inputs:
+        raise ValueError("dense_4bit: rows of shape %s for %d inputs" % (shape, inputs))
     rows = x.size // inputs
-    if x_scale is not None and (x_scale.size != rows or x_scale.dtype != np.float32):
+    if x_scale is not None and (x_scale.size != rows or x_scale.dtype != _F32):
         raise ValueError("dense_4bit: %d scales for %d rows" % (x_scale.size, rows))
-    if bias is not None and (bias.size != outputs or bias.dtype != np.float32):
+    if bias is not None and (bias.size != outputs or bias.dtype != _F32):
         raise ValueError("dense_4bit: bias of %d elements for %d outputs" % (bias.size, outputs))
     if out is None:
-        out = empty(x.shape[:-1] + (outputs,))
-    elif out.size != rows * outputs or out.dtype != np.float32:
-        raise ValueError("dense_4bit: output has shape %s, expected %s" % (out.shape, x.shape[:-1] + (outputs,)))
-    out.take_fresh()
+        out = DeviceArray(shape[:-1] + (outputs,), _F32)
+    elif out.size != rows * outputs or out.dtype != _F32:
+        raise ValueError("dense_4bit: output has shape %s, expected %s" % (out.shape, shape[:-1] + (outputs,)))
+    else:
+        out.take_fresh()
     key = ("dense4", rows, inputs, outputs, x_scale is None)
     need = _NEED.get(key)
     if need is None:

@@ -200,8 +200,14 @@ def rms_norm(x, gamma, eps, residual=None, out=None):
     """(y, s, rstd) over rows of the last axis; s = x + residual, or x itself.  A device ``out`` of the right size
     receives y directly."""
     if is_device(x):
-        y = out if (out is not None and is_device(out) and out.size == x.size) else None
-        return K.rms_norm_fwd(x, same_place(x, gamma).reshape(-1), eps, None if residual is None else same_place(x, residual), y=y)
+        gamma = same_place(x, gamma)
+        if residual is not None:
+            residual = same_place(x, residual)
+        return K.rms_norm_fwd(x, gamma, eps, residual, out if out is not None and is_device(out) and out.size == x.size else None)
+    if not x.ndim or np.size(gamma) != x.shape[-1]:
+        raise ValueError('rms_norm: %d scales for rows of shape %s' % (np.size(gamma), x.shape))
+    if residual is not None and tuple(residual.shape) != x.shape:
+        raise ValueError('rms_norm: residual %s and input %s differ' % (residual.shape, x.shape))
     s = x if residual is None else x + np.asarray(same_place(x, residual))
     rstd = 1 / np.sqrt(np.mean(s * s, axis=-1, keepdims=True) + eps)
     return (s * rstd * np.asarray(same_place(x, gamma)).reshape(-1)).astype(x.dtype, copy=False), s, rstd

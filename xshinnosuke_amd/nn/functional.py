@@ -518,10 +518,6 @@ def rms_norm(inputs, gamma, residual=None, epsilon=1e-6, out=None):
     residual addition takes.  On the device the addition and the normalisation are one pass, and so are their
     backwards.  The backward reads s (``inputs`` without a residual) again: it must not be overwritten in place before."""
     _mark_input(inputs)
-    if residual is not None and tuple(residual.shape) != tuple(inputs.shape):
-        raise ValueError('rms_norm: residual %s and input %s differ' % (residual.shape, inputs.shape))
-    if gamma.eval.size != inputs.shape[-1]:
-        raise ValueError('rms_norm: %d scales for rows of shape %s' % (gamma.eval.size, inputs.shape))
     if not epsilon >= 0:
         raise ValueError('rms_norm: epsilon must not be negative')
     dst = None if out is None else out.eval
@@ -553,13 +549,10 @@ def rms_norm_8bit(inputs, gamma, residual=None, epsilon=1e-6):
     tensors are staged through the device.  Forward only."""
     _mark_input(inputs)
     _forward_only('rms_norm_8bit', inputs, gamma, residual)
-    if residual is not None and tuple(residual.shape) != tuple(inputs.shape):
-        raise ValueError('rms_norm_8bit: residual %s and input %s differ' % (residual.shape, inputs.shape))
     if not epsilon >= 0:
         raise ValueError('rms_norm_8bit: epsilon must not be negative')
     x = inputs.eval
-    q, scale, s = K.rms_norm_int8(_f32_device(x), _f32_device(gamma.eval).reshape(-1), epsilon,
-                                  None if residual is None else _f32_device(residual.eval))
+    q, scale, s = K.rms_norm_int8(_f32_device(x), _f32_device(gamma.eval), epsilon, None if residual is None else _f32_device(residual.eval))
     if not is_device(x):
         q, scale, s = q.numpy(), scale.numpy().astype(x.dtype, copy=False), s.numpy().astype(x.dtype, copy=False)
     return (Tensor(q), Tensor(scale)) if residual is None else (Tensor(q), Tensor(scale), Tensor(s))
@@ -575,11 +568,11 @@ def dense_4bit(inputs, weight, bias=None, scale=None, out=None):
     on_device = is_device(x)
     if scale is not None and x.dtype != np.int8:
         raise ValueError('dense_4bit: rows of %s with a scale, expected int8' % (x.dtype,))
-    if scale is None and np.dtype(x.dtype).kind != 'f':
+    if scale is None and x.dtype.kind != 'f':
         raise ValueError('dense_4bit: rows of %s without a scale' % (x.dtype,))
     x_dev = x if on_device else to_device(np.ascontiguousarray(x), np.float32 if scale is None else np.int8)
     s_dev = None if scale is None else _f32_device(scale.eval)
-    b_dev = None if bias is None else _f32_device(bias.eval).reshape(-1)
+    b_dev = None if bias is None else _f32_device(bias.eval)
     dst = None if out is None else out.eval
     y = weight.product(x_dev, b_dev, s_dev, dst if dst is not None and is_device(dst) else None)
     if out is None:
@@ -594,7 +587,9 @@ def dense_4bit(inputs, weight, bias=None, scale=None, out=None):
 
 
 def _forward_only(what, *tensors):
-    if GLOBAL.COMPUTE_GRAD and any(t is not None and t.requires_grad for t in tensors):
+    if not GLOBAL.COMPUTE_GRAD:
+        return
+    if any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError('%s has no backward: call it under no_grad()' % what)
 
 

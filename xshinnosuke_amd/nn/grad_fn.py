@@ -328,12 +328,16 @@ def _add_rms_norm_grad(src, gamma, dy, rstd):
         if gamma.requires_grad:
             _accumulate(gamma, dgamma)
         return
-    to = [t.grad.eval if t.requires_grad else None for t in (src, gamma)]
-    mine = [a if a is None or is_device(a) else dev.zeros(a.shape, lazy=True) for a in to]
-    K.rms_norm_bwd(A.same_place(s, dy), s, rstd, A.same_place(s, gamma.eval).reshape(-1), dx1=mine[0], dgamma=mine[1])
-    for t, a, b in zip((src, gamma), to, mine):
-        if a is not b:
-            _accumulate(t, b)
+    gamma_dev = A.same_place(s, gamma.eval)
+    dx = src.grad.eval if src.requires_grad else None
+    dg = gamma.grad.eval if gamma.requires_grad else None
+    mine = dx if dx is None or is_device(dx) else dev.zeros(dx.shape, lazy=True)
+    own = dg if dg is None or is_device(dg) else dev.zeros(dg.shape, lazy=True)
+    K.rms_norm_bwd(A.same_place(s, dy), s, rstd, gamma_dev, None, mine, None, own)
+    if mine is not dx:
+        _accumulate(src, mine)
+    if own is not dg:
+        _accumulate(gamma, own)
 
 
 def RMSNormBackward(outputs):
@@ -361,7 +365,7 @@ def ResidualSumBackward(outputs):
     if len(grads) == 2 and fits[0] and fits[1]:
         fits.append(abs(grads[0].address() - grads[1].address()) >= s.nbytes)
     if all(fits):
-        K.rms_norm_bwd(dy, s, rstd, A.same_place(s, gamma.eval).reshape(-1), ds, grads[0], grads[1] if len(grads) == 2 else None, scale)
+        K.rms_norm_bwd(dy, s, rstd, A.same_place(s, gamma.eval), ds, grads[0], grads[1] if len(grads) == 2 else None, scale)
         outputs._grad = None                         # it has never held the normalisation's part
     else:                                            # both addends one tensor, or gradients on the host
         _add_rms_norm_grad(outputs, gamma, dy, rstd)
