@@ -539,7 +539,7 @@ def rms_norm(inputs, gamma, residual=None, epsilon=1e-6, out=None):
     if GLOBAL.COMPUTE_GRAD and out.requires_grad:
         out.cache['rstd'] = rstd
         out.grad_fn = RMSNormBackward
-        initialize_ops_grad(src, gamma)
+        initialize_ops_grad(gamma if residual is not None else src, gamma)      # the sum's gradient is made when something adds to it
     return out if residual is None else (out, src)
 
 

@@ -321,6 +321,7 @@ def BatchNormBackward(outputs):
 def _add_rms_norm_grad(src, gamma, dy, rstd):
     """The gradients of rms_norm's rows and scales, added to theirs."""
     s = src.eval
+    initialize_ops_grad(src)
     if not is_device(s):
         dx, dgamma = A.rms_norm_backward(np.asarray(A.same_place(s, dy)), s, rstd, np.asarray(A.same_place(s, gamma.eval)))
         if src.requires_grad:
@@ -354,10 +355,11 @@ def ResidualSumBackward(outputs):
     """Of s = inputs + residual in rms_norm, with the normalisation's own gradient where that has been left to it."""
     waiting = outputs.cache.pop('normed', None)
     if waiting is None:
-        AddBackward(outputs)
+        if outputs._grad is not None:
+            AddBackward(outputs)
         return
     gamma, dy, rstd = waiting
-    s, ds = outputs.eval, outputs.grad.eval
+    s, ds = outputs.eval, None if outputs._grad is None else outputs.grad.eval
     to = [t for t in outputs.in_bounds if t.requires_grad]
     grads = [t.grad.eval for t in to]
     scale = gamma.grad.eval if gamma.requires_grad else None
