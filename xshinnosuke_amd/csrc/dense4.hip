@@ -530,21 +530,32 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
         // everybody's have; and everybody has read the stage before it, which is loaded anew.
         if (INT8 && p + STAGES - 1 <= pairs) xsmi::wait_vmcnt<LOADS *(STAGES - 2)>(); else xsmi::wait_vmcnt<0>();
         xsmi::block_barrier();
-        if (p + STAGES - 1 < pairs) issue(p + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
         const char *const from = lds + (uint32_t)stage * STAGE;
+        const bool live = 2 * p + half < a.chunks;
+        auto ahead = [&] {
+            if (p + STAGES - 1 < pairs) issue(p + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        };
         Rows x, y;
-        if (INT8) read_weights(from, w); else load_weights(p + 1, next);
-        if (2 * p + half < a.chunks) {
-            read_rows(from, 0, x);
-            if (INT8) {
+        if (INT8) {
+            ahead();
+            read_weights(from, w);
+            if (live) {
+                read_rows(from, 0, x);
                 read_rows(from, 1, y);
                 multiply_i8(w, x, 0);
                 multiply_i8(w, y, 1);
-            } else {
-                h8 v0[NT], v1[NT];
+            }
+        } else {
+            h8 v0[NT], v1[NT];
+            if (live) {
+                read_rows(from, 0, x);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) v0[t] = weights_f16(w.w[t][0]);
                 multiply_f16(w, v0, x, 0, v1, from, y);
+            }
+            ahead();                                 // behind the first multiplications: issuing the loads takes as long as a step
+            load_weights(p + 1, next);
+            if (live) {
                 multiply_f16(w, v1, y, 1, v0, from, x);
                 multiply_f16(w, v0, x, 2, v1, from, y);
                 multiply_f16(w, v1, y, 3, v0, from, x);
