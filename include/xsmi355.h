@@ -472,8 +472,8 @@ int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma
                        float eps);
 /* With a_j = gamma_j dy_j and xhat_j = s_j r: g_j = ds_j + r (a_j - xhat_j mean_i(a_i xhat_i)), dx1 = beta1 dx1 + g,
  * dx2 = beta2 dx2 + g, dgamma_j = beta_gamma dgamma_j + sum over rows of dy_j xhat_j; the betas are 0 or 1.  ds (the
- * gradient that reaches s another way), dx1, dx2 (both addends of s get the same gradient) and dgamma may be NULL; dx1, dx2 and ds may not overlap, but for
- * dx1 == ds.  The workspace is needed for dgamma; the sums are added in an order that depends on the sizes alone. */
+ * gradient that reaches s another way), dx1, dx2 (both addends of s get the same gradient) and dgamma may be NULL; what is written may not overlap what is
+ * read, but for dx1 == ds.  The workspace is needed for dgamma; the sums are added in an order that depends on the sizes alone. */
 size_t xsmi_rms_norm_workspace_bytes(size_t rows, int cols);
 int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const float *gamma, const float *ds, float *dx1, float beta1,
                       float *dx2, float beta2, float *dgamma, float beta_gamma, size_t rows, int cols, void *ws, size_t ws_bytes);

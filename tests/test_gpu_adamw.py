@@ -190,6 +190,29 @@ def test_moving_between_host_and_device_keeps_the_moments():
     _check_parameters([p], [plain], [change], 5)
 
 
+def test_a_lot_of_host_and_new_parameters_moves_to_the_device():
+    """Parameters with and without steps behind them, all on the device from now on: each keeps its own count."""
+    rng = np.random.default_rng(17)
+    values = [rng.standard_normal(n).astype(np.float32) for n in (7, 300, 11)]
+    params = [xs.Parameter(xs.Tensor(v.copy(), requires_grad=True)) for v in values]
+    plain = [Plain(v) for v in values]
+    opt, changes = AdamW(params), [0.0] * 3
+    for step in range(4):
+        if step == 2:
+            for p in params:
+                p.cuda_()
+            xs.GLOBAL.USE_CUDA = False
+        for i, (p, q) in enumerate(zip(params, plain)):
+            if i == 2 and step < 2:
+                continue
+            g = _gradient(rng, p.shape)
+            p.grad = xs.Tensor(be.to_device(g) if step >= 2 else g)
+            changes[i] = max(changes[i], np.abs(q.step(g)).max())
+        opt.step()
+    _check_parameters(params, plain, changes, 4)
+    assert sorted(len(g[0]) for g in opt.moments()) == [1, 2]
+
+
 def test_new_parameters_and_gradients_start_their_own_count():
     rng = np.random.default_rng(8)
     params, _, _ = _params([rng.standard_normal(n).astype(np.float32) for n in (10, 20)])

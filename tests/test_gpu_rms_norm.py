@@ -171,6 +171,37 @@ def test_one_tensor_as_both_addends():
         assert np.abs(a.grad.numpy() - b.grad.numpy()).max() <= 100 * EPS * np.abs(b.grad.numpy()).max()
 
 
+def test_several_normalisations_of_one_sum():
+    """The stream that one norm returns goes through another norm of its own, and on."""
+    rng = np.random.default_rng(13)
+    x, r, gamma, dy, _ = _case(rng, 6, 50)
+    grads = []
+    for device in (True, False):
+        tensor = (lambda a, **k: _dev(a, **k)) if device else (lambda a, **k: xs.Tensor(a.astype(np.float64), **k))
+        tx, tr = tensor(x, requires_grad=True), tensor(r, requires_grad=True)
+        gammas = [xs.Parameter(tensor(gamma + k, requires_grad=True)) for k in range(3)]
+        y, s = F.rms_norm(tx, gammas[0], tr)
+        z = F.rms_norm(s, gammas[1]) + F.rms_norm(s, gammas[2])
+        (z + y + s).backward(tensor(dy))
+        grads.append([t.grad.numpy() for t in (tx, tr, *gammas)])
+    for a, b in zip(*grads):
+        assert np.abs(a - b).max() <= 4 * _roundings(6, 50) * EPS * np.abs(b).max()
+
+
+def test_more_rows_than_one_launch_takes():
+    rng = np.random.default_rng(14)
+    rows = (1 << 21) + 5
+    x, r, gamma, _, _ = _case(rng, rows, 2)
+    with xs.no_grad():
+        y, s = F.rms_norm(_dev(x), _dev(gamma), _dev(r))
+        q, scale, _ = F.rms_norm_8bit(_dev(x), _dev(gamma), _dev(r))
+    w = (x + r).astype(np.float64)
+    want = w / np.sqrt((w * w).mean(1, keepdims=True) + 1e-6) * gamma
+    assert np.array_equal(s.numpy(), x + r) and np.all(np.abs(y.numpy() - want) <= _roundings(1, 2) * EPS * np.abs(want))
+    most = np.abs(want).max(1)
+    assert np.all(np.abs(q.numpy() - want * (127 / most)[:, None]) <= 0.5 + 1e-9) and np.allclose(scale.numpy(), most / 127, rtol=2 * EPS)
+
+
 def test_only_the_scales_or_only_the_rows_want_a_gradient():
     rng = np.random.default_rng(11)
     x, r, gamma, dy, _ = _case(rng, 5, 70)

@@ -68,6 +68,15 @@ def test_fit_save_load_and_go_on(tmp_path):
     assert a['train_loss'] == b['train_loss'] and again.optimizer.iterations == net.optimizer.iterations == 12
 
 
+def test_a_parameter_of_another_size_is_refused():
+    p = _param(np.ones(3), np.ones(3))
+    opt = AdamW([p])
+    opt.step()
+    p._data, p.grad = np.ones(4), xs.Tensor(np.ones(4))
+    with pytest.raises(ValueError):
+        opt.step()
+
+
 def test_refusals():
     p = _param(np.ones(3), np.ones(3))
     for bad in (dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(betas=(0.9,)), dict(lr=-1), dict(lr=float('nan')), dict(epsilon=-1e-8),

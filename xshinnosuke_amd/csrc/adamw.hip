@@ -23,6 +23,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef f4 f4u __attribute__((aligned(4)));              // parameters and gradients may start at any element
 constexpr int MAX_TENSORS = 96;                          // of one launch: its arguments stay below 4 KB
 constexpr int BLOCK = 256;                               // elements that share an exponent
+constexpr uint64_t MAX_GROUPS = (1u << 24) - 1;          // workgroups of 256 threads in a launch
 
 // What a step needs beside its tensors, moved by the launch in front of it (device memory of the caller).
 struct StepState {
@@ -303,7 +304,7 @@ int xsmi_adamw_step(int count, float *const *ps, const float *const *gs, const s
         XSMI_CHECK_ARG(ps[i] && gs[i], "xsmi_adamw_step: null pointer in tensor %d", i);
         XSMI_CHECK_ARG(starts[i] % BLOCK == 0 && starts[i] <= moments && ns[i] <= moments - starts[i],
                        "xsmi_adamw_step: tensor %d has its moments at %zu of %zu", i, starts[i], moments);
-        XSMI_CHECK_ARG(ns[i] < (1ull << 40), "xsmi_adamw_step: tensor %d too large", i);
+        XSMI_CHECK_ARG(ns[i] < 1024ull * MAX_GROUPS, "xsmi_adamw_step: tensor %d has %zu elements", i, ns[i]);
     }
     XSMI_CHECK_ARG(moments % BLOCK == 0, "xsmi_adamw_step: room for %zu moments, expected a multiple of %d", moments, BLOCK);
     hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(1), 0, xsmi::stream(), (StepState *)state, lr, beta1, beta2, seed);
@@ -320,13 +321,13 @@ int xsmi_adamw_step(int count, float *const *ps, const float *const *gs, const s
         for (; done < count && k < MAX_TENSORS; ++done) {
             if (ns[done] == 0) continue;
             const uint64_t more = (ns[done] + 1023u) / 1024u;
-            if (groups + more > 0x7fffffffull) break;
+            if (groups + more > MAX_GROUPS) break;
             t.p[k] = ps[done], t.g[k] = gs[done], t.start[k] = starts[done], t.n[k] = ns[done];
             t.first[k++] = (uint32_t)groups;
             groups += more;
         }
         t.count = k;
-        if (k == 0) break;
+        if (k == 0) break;                               // nothing but empty tensors was left
 #define LAUNCH(kernel, ...) hipLaunchKernelGGL((kernel), dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), t, __VA_ARGS__, f, (const StepState *)state)
         if (state_bits == 32) {
             if (stream) LAUNCH((adamw_kernel<true>), (float *)m, (float *)v);
@@ -348,7 +349,7 @@ int xsmi_adamw_moments(const uint8_t *m8, const uint8_t *v8, const uint8_t *m_ex
     XSMI_CHECK_ARG(moments % BLOCK == 0, "xsmi_adamw_moments: %zu moments, expected a multiple of %d", moments, BLOCK);
     XSMI_CHECK_ARG((((uintptr_t)m | (uintptr_t)v) & 15) == 0 && (((uintptr_t)m8 | (uintptr_t)v8) & 3) == 0, "xsmi_adamw_moments: unaligned moments");
     const uint64_t groups = (moments + 1023) / 1024;
-    XSMI_CHECK_ARG(groups < (1ull << 31), "xsmi_adamw_moments: too many moments");
+    XSMI_CHECK_ARG(groups <= MAX_GROUPS, "xsmi_adamw_moments: %zu moments", moments);
     const Moments8 q = {(uint8_t *)m8, (uint8_t *)v8, (uint8_t *)m_exp, (uint8_t *)v_exp};
     if ((double)moments * 10 > 256e6) hipLaunchKernelGGL(adamw_moments_kernel<true>, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), q, m, v, (uint64_t)moments);
     else hipLaunchKernelGGL(adamw_moments_kernel<false>, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), q, m, v, (uint64_t)moments);

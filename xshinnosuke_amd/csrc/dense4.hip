@@ -641,8 +641,11 @@ __global__ void __launch_bounds__(256) dequantize4_kernel(const uint8_t *__restr
 
 inline int up(int v, int to) { return (v + to - 1) / to * to; }
 
+// 2^24 inputs or outputs: launches and offsets inside a chunk count in 32 bits.
+inline bool sizes_ok(int K, int N) { return K >= 1 && N >= 1 && K <= (1 << 24) && N <= (1 << 24); }
+
 int check_weights(const char *who, int K, int N, int group) {
-    XSMI_CHECK_ARG(K >= 1 && N >= 1 && K <= (1 << 30) && N <= (1 << 30), "%s: %d inputs, %d outputs", who, K, N);
+    XSMI_CHECK_ARG(sizes_ok(K, N), "%s: %d inputs, %d outputs", who, K, N);
     XSMI_CHECK_ARG(group == 32 || group == 64 || group == 128, "%s: groups of %d inputs, expected 32, 64 or 128", who, group);
     return XSMI_OK;
 }
@@ -702,17 +705,17 @@ int launch(const Dense &a, void *ws) {
 extern "C" {
 
 size_t xsmi_dense_4bit_code_bytes(int K, int N) {
-    if (K < 1 || N < 1 || K > (1 << 30) || N > (1 << 30)) return 0;
+    if (!sizes_ok(K, N)) return 0;
     return (size_t)up(K, 128) * up(N, 16) / 2;
 }
 
 size_t xsmi_dense_4bit_scale_count(int K, int N, int group) {
-    if (K < 1 || N < 1 || K > (1 << 30) || N > (1 << 30) || (group != 32 && group != 64 && group != 128)) return 0;
+    if (!sizes_ok(K, N) || (group != 32 && group != 64 && group != 128)) return 0;
     return (size_t)(up(K, 128) / group) * up(N, 16);
 }
 
 size_t xsmi_dense_4bit_workspace_bytes(size_t M, int K, int N, int x_bits) {
-    if (K < 1 || N < 1 || K > (1 << 30) || N > (1 << 30) || (x_bits != 8 && x_bits != 32) || M >= (1u << 21) || few(M, x_bits == 8)) return 0;
+    if (!sizes_ok(K, N) || (x_bits != 8 && x_bits != 32) || M >= (1u << 21) || few(M, x_bits == 8)) return 0;
     return (size_t)up((int)M, BLOCK_ROWS) * (4 + (size_t)up(K, 128) * (x_bits == 8 ? 1 : 4));
 }
 
@@ -723,7 +726,7 @@ int xsmi_quantize_4bit(const float *w, int K, int N, int group, uint8_t *codes, 
     XSMI_CHECK_ARG(((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 7) == 0, "xsmi_quantize_4bit: unaligned codes or scales");
     const int chunks = up(K, 128) / 128, cols = up(N, 16);
     const uint64_t groups = (uint64_t)(cols / 16) * chunks;
-    XSMI_CHECK_ARG(groups < (1ull << 31), "xsmi_quantize_4bit: %d x %d weights", K, N);
+    XSMI_CHECK_ARG(groups < (1u << 24), "xsmi_quantize_4bit: %d x %d weights", K, N);
     hipLaunchKernelGGL(quantize4_kernel, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), w, codes, (_Float16 *)scales, K, N, group, chunks, cols);
     XSMI_LAUNCH_CHECK("quantize4_kernel");
     return XSMI_OK;
@@ -734,7 +737,7 @@ int xsmi_dequantize_4bit(const uint8_t *codes, const void *scales, int K, int N,
     if (int rc = check_weights("xsmi_dequantize_4bit", K, N, group)) return rc;
     XSMI_CHECK_ARG(w && codes && scales, "xsmi_dequantize_4bit: null pointer");
     const uint64_t groups = ((uint64_t)K * N + 255) / 256;
-    XSMI_CHECK_ARG(groups < (1ull << 31), "xsmi_dequantize_4bit: %d x %d weights", K, N);
+    XSMI_CHECK_ARG(groups < (1u << 24), "xsmi_dequantize_4bit: %d x %d weights", K, N);
     hipLaunchKernelGGL(dequantize4_kernel, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), codes, (const _Float16 *)scales, w, K, N, group, up(K, 128) / 128, up(N, 16));
     XSMI_LAUNCH_CHECK("dequantize4_kernel");
     return XSMI_OK;

@@ -406,6 +406,18 @@ __global__ void __launch_bounds__(1024) rms_dgamma_kernel(const float *__restric
 
 constexpr uint64_t MAX_ROWS = 1ull << 31;
 
+constexpr size_t LAUNCH_ROWS = 1u << 21;             // of one launch: its threads count in 32 bits
+Forward lot(Forward a, size_t first) {
+    const uint64_t at = first * (uint64_t)a.cols;
+    a.x += at;
+    a.rows = a.rows - first < LAUNCH_ROWS ? a.rows - first : LAUNCH_ROWS;
+    if (a.residual) a.residual += at, a.sum += at;
+    if (a.y) a.y += at;
+    if (a.rstd) a.rstd += first;
+    if (a.q) a.q += at, a.scale += first;
+    return a;
+}
+
 // Workgroups of the backward, and the rows of part that they write.
 struct BackwardPlan {
     int threads_a_row, threads, groups, parts;
@@ -456,16 +468,19 @@ int xsmi_rms_norm_fwd(const float *x, const float *residual, const float *gamma,
     if (int rc = check("xsmi_rms_norm_fwd", rows, cols, eps)) return rc;
     if (rows == 0) return XSMI_OK;
     XSMI_CHECK_ARG(x && gamma && y && (residual == nullptr) == (sum == nullptr), "xsmi_rms_norm_fwd: null pointer (a residual comes with a sum)");
-    const Forward a = {x, residual, gamma, sum, y, rstd, nullptr, nullptr, rows, cols, eps};
     const bool stream = streams(rows, cols, residual ? 4 : 2);
     const int need = (cols + 3) / 4;
-    if (need <= 16) LAUNCH_TWO(rms_fwd_kernel, 16, 256, 1, (rows + 15) / 16, a);
-    else if (need <= 64) LAUNCH_TWO(rms_fwd_kernel, 64, 256, 1, (rows + 3) / 4, a);
-    else if (need <= 256) LAUNCH_TWO(rms_fwd_kernel, 256, 256, 1, rows, a);
-    else if (need <= 1024) LAUNCH_TWO(rms_fwd_kernel, 512, 512, 2, rows, a);
-    else if (need <= 4096) LAUNCH_TWO(rms_fwd_kernel, 1024, 1024, 4, rows, a);
-    else LAUNCH((rms_fwd_long_kernel<1024>), rows, 1024, a);
-    XSMI_LAUNCH_CHECK("rms_fwd_kernel");
+    for (size_t first = 0; first < rows; first += LAUNCH_ROWS) {
+        const Forward a = lot({x, residual, gamma, sum, y, rstd, nullptr, nullptr, rows, cols, eps}, first);
+        const size_t n = a.rows;
+        if (need <= 16) LAUNCH_TWO(rms_fwd_kernel, 16, 256, 1, (n + 15) / 16, a);
+        else if (need <= 64) LAUNCH_TWO(rms_fwd_kernel, 64, 256, 1, (n + 3) / 4, a);
+        else if (need <= 256) LAUNCH_TWO(rms_fwd_kernel, 256, 256, 1, n, a);
+        else if (need <= 1024) LAUNCH_TWO(rms_fwd_kernel, 512, 512, 2, n, a);
+        else if (need <= 4096) LAUNCH_TWO(rms_fwd_kernel, 1024, 1024, 4, n, a);
+        else LAUNCH((rms_fwd_long_kernel<1024>), n, 1024, a);
+        XSMI_LAUNCH_CHECK("rms_fwd_kernel");
+    }
     return XSMI_OK;
 }
 
@@ -475,15 +490,18 @@ int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma
     if (int rc = check("xsmi_rms_norm_int8", rows, cols, eps)) return rc;
     if (rows == 0) return XSMI_OK;
     XSMI_CHECK_ARG(x && gamma && q && scale && (residual == nullptr) == (sum == nullptr), "xsmi_rms_norm_int8: null pointer (a residual comes with a sum)");
-    const Forward a = {x, residual, gamma, sum, nullptr, nullptr, q, scale, rows, cols, eps};
     const int need = (cols + 3) / 4;
-    if (need <= 16) LAUNCH((rms_fwd_int8_kernel<16, 256, 1>), (rows + 15) / 16, 256, a);
-    else if (need <= 64) LAUNCH((rms_fwd_int8_kernel<64, 256, 1>), (rows + 3) / 4, 256, a);
-    else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1>), rows, 256, a);
-    else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 1>), rows, 1024, a);
-    else if (need <= 4096) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 4>), rows, 1024, a);
-    else LAUNCH((rms_fwd_int8_long_kernel<1024>), rows, 1024, a);
-    XSMI_LAUNCH_CHECK("rms_fwd_int8_kernel");
+    for (size_t first = 0; first < rows; first += LAUNCH_ROWS) {
+        const Forward a = lot({x, residual, gamma, sum, nullptr, nullptr, q, scale, rows, cols, eps}, first);
+        const size_t n = a.rows;
+        if (need <= 16) LAUNCH((rms_fwd_int8_kernel<16, 256, 1>), (n + 15) / 16, 256, a);
+        else if (need <= 64) LAUNCH((rms_fwd_int8_kernel<64, 256, 1>), (n + 3) / 4, 256, a);
+        else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1>), rows, 256, a);
+        else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 1>), n, 1024, a);
+        else if (need <= 4096) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 4>), n, 1024, a);
+        else LAUNCH((rms_fwd_int8_long_kernel<1024>), n, 1024, a);
+        XSMI_LAUNCH_CHECK("rms_fwd_int8_kernel");
+    }
     return XSMI_OK;
 }
 

@@ -344,8 +344,10 @@ def _add_rms_norm_grad(src, gamma, dy, rstd):
 def RMSNormBackward(outputs):
     src, gamma = outputs.in_bounds
     dy, rstd = outputs.grad.eval, outputs.cache['rstd']
-    if src.grad_fn is ResidualSumBackward and is_device(src.eval) and is_device(dy) and not src.retain_grad():
-        # s = x + residual is next but one at the latest: its own gradient is whole by then, and both go to the addends in one pass
+    if (src.grad_fn is ResidualSumBackward and 'normed' not in src.cache and is_device(src.eval) and is_device(dy)
+            and not src.retain_grad()):
+        # s = x + residual comes after all that use it: its own gradient is whole by then, and both go to the addends in one pass
+        # (of several normalisations of one sum, the first one's)
         src.cache['normed'] = (gamma, dy, rstd)
     else:
         _add_rms_norm_grad(src, gamma, dy, rstd)

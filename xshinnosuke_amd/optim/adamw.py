@@ -24,10 +24,10 @@ class _DeviceMoments:
         if dev._CAPTURE[0] is not None:
             raise XsmiError("AdamW's moments must exist before a step is recorded: run one step first")
         self.params, self.bits = list(params), bits
-        self.starts, total = [], 0
-        for p in self.params:
+        self.sizes, self.starts, total = [p._data.size for p in self.params], [], 0
+        for size in self.sizes:
             self.starts.append(total)
-            total += -(-p._data.size // 256) * 256
+            total += -(-size // 256) * 256
         total = max(total, 256)
         kind = np.float32 if bits == 32 else np.uint8
         self.m, self.v = dev.zeros((total,), kind), dev.zeros((total,), kind)
@@ -35,9 +35,9 @@ class _DeviceMoments:
         if bits == 8:
             self.me, self.ve = dev.zeros((total // 256,), np.uint8), dev.zeros((total // 256,), np.uint8)
         self.state = dev.to_device(np.array([steps, 0, 0], np.int64))
-        for start, p, pair in zip(self.starts, self.params, values or ()):
+        for start, size, pair in zip(self.starts, self.sizes, values or ()):
             for flat, value in zip((self.m, self.v), pair):
-                flat.leading(start, start + p._data.size).set(np.asarray(value, np.float32).reshape(-1))
+                flat.leading(start, start + size).set(np.asarray(value, np.float32).reshape(-1))
         self.launch = None
 
     def __getstate__(self):
@@ -58,7 +58,7 @@ class _Launch:
         self.of = []                                  # (parameter, its array, gradient tensor, its array)
         values, grads, starts = [], [], []
         self.lasting = True
-        for p, start in zip(moments.params, moments.starts):
+        for p, start, size in zip(moments.params, moments.starts, moments.sizes):
             if p is None or p._grad is None or not p.requires_grad:
                 self.lasting = False
                 continue
@@ -66,9 +66,11 @@ class _Launch:
             if not A.is_device(grad) or value is not p._data or grad is not p._grad._data:
                 self.lasting = False
             grad = A.same_place(value, grad)
-            if value.size > -(-p._data.size // 256) * 256 or value.size != grad.size or value.dtype != np.float32 or grad.dtype != np.float32:
+            if value.size != grad.size or value.dtype != np.float32 or grad.dtype != np.float32:
                 raise ValueError("AdamW: parameter %s %s and gradient %s %s: both must be float32, of one size"
                                  % (value.shape, value.dtype, grad.shape, grad.dtype))
+            if value.size > size:
+                raise ValueError("AdamW: parameter %s has moments of %d elements" % (value.shape, size))
             self.of.append((p, value, p._grad, grad))
             values.append(value)
             grads.append(grad)
@@ -140,12 +142,12 @@ class AdamW(Optimizer):
                     if self.state_bits == 8:
                         raise NotImplementedError('AdamW: 8-bit moments need device tensors')
                     self._host[p] = [np.zeros_like(p._data), np.zeros_like(p._data), 0]
-        moved = {}
+        lots = {}                                     # by steps taken: those of a parameter that comes from the host go on
         for p in fresh:
-            moved.setdefault(self._host[p][2] if p in self._host else 0, []).append(p)
-        for steps, params in moved.items():
-            values = [tuple(self._host.pop(p)[:2]) for p in params] if params[0] in self._host else None
-            self._groups.append(_DeviceMoments(params, self.state_bits, steps, values))
+            m, v, steps = self._host.pop(p, (np.zeros(p._data.size, np.float32),) * 2 + (0,))
+            lots.setdefault(steps, []).append((p, (m, v)))
+        for steps, lot in lots.items():
+            self._groups.append(_DeviceMoments([p for p, _ in lot], self.state_bits, steps, [pair for _, pair in lot] if steps else None))
         return host
 
     def _fetch(self, p, group):
@@ -153,7 +155,9 @@ class AdamW(Optimizer):
         if group.bits == 8:
             raise NotImplementedError('AdamW: 8-bit moments need device tensors')
         i = [q is p for q in group.params].index(True)
-        stretch = slice(group.starts[i], group.starts[i] + p._data.size)
+        if p._data.size != group.sizes[i]:
+            raise ValueError('AdamW: parameter %s has moments of %d elements' % (p._data.shape, group.sizes[i]))
+        stretch = slice(group.starts[i], group.starts[i] + group.sizes[i])
         self._host[p] = [np.asarray(a)[stretch].reshape(p._data.shape).astype(p._data.dtype) for a in (group.m, group.v)] + [group.steps()]
         group.params[i] = group.launch = None
 
