@@ -361,15 +361,17 @@ def ResidualSumBackward(outputs):
             AddBackward(outputs)
         return
     gamma, dy, rstd = waiting
-    s, ds = outputs.eval, None if outputs._grad is None else outputs.grad.eval
-    to = [t for t in outputs.in_bounds if t.requires_grad]
-    grads = [t.grad.eval for t in to]
+    a, b = outputs._in_bounds
+    first = a.grad.eval if a.requires_grad else None
+    second = b.grad.eval if b.requires_grad else None
+    if first is None:
+        first, second = second, None
     scale = gamma.grad.eval if gamma.requires_grad else None
-    fits = [is_device(a) and a.dtype == np.float32 and a.size == s.size for a in grads] + [scale is None or is_device(scale)]
-    if len(grads) == 2 and fits[0] and fits[1]:
-        fits.append(abs(grads[0].address() - grads[1].address()) >= s.nbytes)
-    if all(fits):
-        K.rms_norm_bwd(dy, s, rstd, A.same_place(s, gamma.eval), ds, grads[0], grads[1] if len(grads) == 2 else None, scale)
+    if (is_device(first) and (scale is None or is_device(scale)) and
+            (second is None or (is_device(second) and (second._block is not first._block or
+                                                       abs(first.address() - second.address()) >= first.nbytes)))):
+        s = outputs.eval
+        K.rms_norm_bwd(dy, s, rstd, A.same_place(s, gamma.eval), None if outputs._grad is None else outputs.grad.eval, first, second, scale)
         outputs._grad = None                         # it has never held the normalisation's part
     else:                                            # both addends one tensor, or gradients on the host
         _add_rms_norm_grad(outputs, gamma, dy, rstd)
