@@ -461,6 +461,7 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
     auto multiply_f16 = [&](const Weights &r, const h8 *w, const Rows &x, int step, h8 *w_next, const char *stage, Rows &x_next) {
         if (step < 3) read_rows(stage, step + 1, x_next);
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);               // the wave that multiplies goes before the one that makes ready: 39.8 -> 39.2 us
         if (step < 3) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) w_next[t] = weights_f16(r.w[t][step + 1]);
@@ -481,6 +482,7 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
                 __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);       // vector
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
         if ((step + 1) % (G / 32) == 0) {
 #pragma unroll
