@@ -388,13 +388,14 @@ __global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, char *operand
 // and scales into registers; 8-bit rows, which are multiplied faster than a load comes back, leave room for four stages with
 // codes and scales.
 template <int G, bool INT8>
-__global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char *operand, const float *back) {
+__global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char *operand, const float *back, float *part, int each) {
     constexpr uint32_t ROWS = piece_bytes(INT8), STAGE = many_stage_bytes(INT8);
     constexpr int STAGES = many_stages(INT8), LOADS = 2 * ROWS / 8192 + (INT8 ? 4 : 0);      // of a wave for a stage, straight into LDS
     constexpr int GROUPS = 128 / G, NT = 2, MT = 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, col = lane & 15;
-    const int tiles = a.cols / 16, t0 = blockIdx.x * 8, n_wave = (wave & 3) * NT, half = wave >> 2, pairs = (a.chunks + 1) / 2;
+    const int tiles = a.cols / 16, t0 = blockIdx.x * 8, n_wave = (wave & 3) * NT, half = wave >> 2;
+    const int p0 = blockIdx.z * each, pairs = min((a.chunks + 1) / 2, p0 + each);      // this workgroup's pairs of chunks
     const char *const block = operand + (uint64_t)blockIdx.y * a.chunks * ROWS;
     const uint8_t *const own_codes = a.codes + (uint64_t)min(t0 + wave, tiles - 1) * a.chunks * 1024;
     const uint32_t lds0 = (uint32_t)(uintptr_t)&lds[0];
@@ -524,10 +525,10 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
     Weights w, next;
 #pragma unroll
     for (int p = 0; p < STAGES - 1; ++p)
-        if (p < pairs) issue(p, p);
-    if (!INT8) load_weights(0, w);
+        if (p0 + p < pairs) issue(p0 + p, p);
+    if (!INT8) load_weights(p0, w);
     int stage = 0;
-    for (int p = 0; p < pairs; ++p) {
+    for (int p = p0; p < pairs; ++p) {
         // This wave's loads of the stage have arrived (no more than the later stages' are under way) and, behind the barrier,
         // everybody's have; and everybody has read the stage before it, which is loaded anew.
         if (INT8 && p + STAGES - 1 <= pairs) xsmi::wait_vmcnt<LOADS *(STAGES - 2)>(); else xsmi::wait_vmcnt<0>();
@@ -582,6 +583,13 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
     for (int u = 0; u < MT; ++u) {
         const int m = blockIdx.y * BLOCK_ROWS + u * 16 + col;
         if (m >= a.M) continue;
+        if (part) {                                  // one of several workgroups for these results: the sums as they are
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if ((t0 + n_wave + t) * 16 < a.cols)
+                    *reinterpret_cast<f4 *>(part + ((uint64_t)blockIdx.z * a.M + m) * a.cols + (t0 + n_wave + t) * 16 + 4 * q) = acc[t][u] + other[(t * MT + u) * 64];
+            continue;
+        }
         const float f = INT8 ? a.x_scale[m] * 0.0625f : back[m];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -598,6 +606,20 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
             }
         }
     }
+}
+
+// The sums of a result's workgroups, in order of their inputs.
+template <bool INT8>
+__global__ void __launch_bounds__(256) dense4_join_kernel(Dense a, const float *__restrict__ part, const float *__restrict__ back, int splits) {
+    const int m = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (n >= a.N) return;
+    f4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int z = 0; z < splits; ++z) y += *reinterpret_cast<const f4 *>(part + ((uint64_t)z * a.M + m) * a.cols + n);
+    y *= INT8 ? a.x_scale[m] * 0.0625f : back[m];
+    float *const to = a.y + (uint64_t)m * a.N + n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < a.N) to[e] = a.bias ? y[e] + a.bias[n + e] : y[e];
 }
 
 // ---- the weights -------------------------------------------------------------------------------------------------
@@ -652,6 +674,22 @@ int check_weights(const char *who, int K, int N, int group) {
     return XSMI_OK;
 }
 
+// Many rows: where the results make fewer workgroups than there are compute units, the inputs are split among several, of two pairs of
+// chunks at least, and their sums joined by a launch of its own (64 rows, 4096 x 4096: 34 us on 32 workgroups, 20 on 256).
+struct Split {
+    int splits, pairs;                               // pairs of chunks of each
+};
+inline Split split_of(int M, int K, int N) {
+    const int64_t groups = (int64_t)((up(N, 16) + 127) / 128) * ((M + 63) / 64);
+    const int pairs = (up(K, 128) / 128 + 1) / 2;
+    int splits = groups >= 256 ? 1 : (int)(256 / groups);
+    if (splits > pairs / 2) splits = pairs / 2;
+    if (splits > 16) splits = 16;
+    if (splits < 1) splits = 1;
+    const int each = (pairs + splits - 1) / splits;
+    return Split{(pairs + each - 1) / each, each};
+}
+
 // Few rows: those whose digits fit four tiles of columns.
 inline bool few(size_t M, bool int8) { return M <= (int8 ? 64u : 16u); }
 
@@ -692,13 +730,19 @@ int launch_few(const Dense &a) {
 template <int G, bool INT8>
 int launch(const Dense &a, void *ws) {
     if (few(a.M, INT8)) return launch_few<G, INT8 ? 1 : 4>(a);
+    const Split split = split_of(a.M, a.K, a.N);
     float *const back = (float *)ws;
     char *const operand = (char *)ws + up(a.M, BLOCK_ROWS) * 4;
+    float *const part = split.splits > 1 ? (float *)(operand + (size_t)up(a.M, BLOCK_ROWS) * a.chunks * 128 * (INT8 ? 1 : 4)) : nullptr;
     hipLaunchKernelGGL(dense4_rows_kernel<INT8>, dim3(a.M), dim3(256), 0, xsmi::stream(), a, operand, back);
     XSMI_LAUNCH_CHECK("dense4_rows_kernel");
-    hipLaunchKernelGGL((dense4_many_kernel<G, INT8>), dim3((a.cols + 127) / 128, (a.M + BLOCK_ROWS - 1) / BLOCK_ROWS), dim3(512), many_lds_bytes(INT8), xsmi::stream(),
-                       a, (const char *)operand, (const float *)back);
+    hipLaunchKernelGGL((dense4_many_kernel<G, INT8>), dim3((a.cols + 127) / 128, (a.M + BLOCK_ROWS - 1) / BLOCK_ROWS, split.splits), dim3(512), many_lds_bytes(INT8),
+                       xsmi::stream(), a, (const char *)operand, (const float *)back, part, split.pairs);
     XSMI_LAUNCH_CHECK("dense4_many_kernel");
+    if (part) {
+        hipLaunchKernelGGL(dense4_join_kernel<INT8>, dim3((a.cols + 1023) / 1024, a.M), dim3(256), 0, xsmi::stream(), a, (const float *)part, (const float *)back, split.splits);
+        XSMI_LAUNCH_CHECK("dense4_join_kernel");
+    }
     return XSMI_OK;
 }
 
@@ -718,7 +762,8 @@ size_t xsmi_dense_4bit_scale_count(int K, int N, int group) {
 
 size_t xsmi_dense_4bit_workspace_bytes(size_t M, int K, int N, int x_bits) {
     if (!sizes_ok(K, N) || (x_bits != 8 && x_bits != 32) || M >= (1u << 21) || few(M, x_bits == 8)) return 0;
-    return (size_t)up((int)M, BLOCK_ROWS) * (4 + (size_t)up(K, 128) * (x_bits == 8 ? 1 : 4));
+    const int splits = split_of((int)M, K, N).splits;
+    return (size_t)up((int)M, BLOCK_ROWS) * (4 + (size_t)up(K, 128) * (x_bits == 8 ? 1 : 4)) + (splits > 1 ? (size_t)splits * M * up(N, 16) * 4 : 0);
 }
 
 int xsmi_quantize_4bit(const float *w, int K, int N, int group, uint8_t *codes, void *scales) {
@@ -751,7 +796,7 @@ int xsmi_dense_4bit(const void *x, const float *x_scale, const uint8_t *codes, c
     if (int rc = check_weights("xsmi_dense_4bit", K, N, group)) return rc;
     if (M == 0) return XSMI_OK;
     XSMI_CHECK_ARG(x && codes && scales && y, "xsmi_dense_4bit: null pointer");
-    XSMI_CHECK_ARG(M < (1u << 21), "xsmi_dense_4bit: %zu rows", M);
+    XSMI_CHECK_ARG(M < (1u << 21), "xsmi_dense_4bit: %zu rows", M);      // 64 rows of a workgroup in one direction of the launch, one in another
     XSMI_CHECK_ARG(((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 7) == 0 && ((uintptr_t)ws & 15) == 0, "xsmi_dense_4bit: unaligned codes, scales or workspace");
     const bool int8 = x_scale != nullptr;
     const size_t want = xsmi_dense_4bit_workspace_bytes(M, K, N, int8 ? 8 : 32);
