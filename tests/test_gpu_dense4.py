@@ -40,7 +40,7 @@ def _tolerance(x, w, group, whole=False):
     return ((group + groups + 12) * EPS + 2.0 ** -22) * size + 2.0 ** -28 * np.abs(x).max(1, keepdims=True) * np.abs(w).sum(0)
 
 
-ROWS = [1, 2, 3, 4, 5, 8, 9, 16, 17, 33, 64, 65, 130]
+ROWS = [1, 2, 3, 4, 5, 8, 9, 13, 16, 17, 33, 48, 49, 64, 65, 130]
 SHAPES = [(1, 1), (7, 3), (32, 16), (127, 17), (128, 15), (129, 100), (512, 1000), (1000, 33), (2177, 40), (9001, 19), (20000, 5)]
 
 

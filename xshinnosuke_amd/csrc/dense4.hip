@@ -690,8 +690,14 @@ inline Split split_of(int M, int K, int N) {
     return Split{(pairs + each - 1) / each, each};
 }
 
-// Few rows: those whose digits fit four tiles of columns.
-inline bool few(size_t M, bool int8) { return M <= (int8 ? 64u : 16u); }
+// Few rows: those whose digits fit two tiles of columns, and up to four tiles where a wave goes through less than eight windows: each
+// takes some 3 us then, and the many rows' kernels 12 us and more in all (16 rows, 8192 x 2048: 27.0 us as few, 19.4 as
+// many; 12 rows, 4096 x 4096: 13.5 and 16; 64 rows of 8 bits, 8192 x 8192: 26.2 and 20.3; 43, 5000 x 7001: 18.2 and 20.4).
+inline bool few(size_t M, int K, int N, bool int8) {
+    if (M <= (int8 ? 32u : 8u)) return true;
+    const int windows = (up(K, 128) / 128 + WAVES - 1) / WAVES, rounds = (up(N, 32) / 32 + 255) / 256;
+    return M <= (int8 ? 64u : 16u) && (int64_t)windows * rounds < 8;
+}
 
 // ROWS: the most that there may be.
 template <int G, int DIGITS, int ROWS, int NT, int PF, bool LOOP>
@@ -729,7 +735,7 @@ int launch_few(const Dense &a) {
 
 template <int G, bool INT8>
 int launch(const Dense &a, void *ws) {
-    if (few(a.M, INT8)) return launch_few<G, INT8 ? 1 : 4>(a);
+    if (few(a.M, a.K, a.N, INT8)) return launch_few<G, INT8 ? 1 : 4>(a);
     const Split split = split_of(a.M, a.K, a.N);
     float *const back = (float *)ws;
     char *const operand = (char *)ws + up(a.M, BLOCK_ROWS) * 4;
@@ -761,7 +767,7 @@ size_t xsmi_dense_4bit_scale_count(int K, int N, int group) {
 }
 
 size_t xsmi_dense_4bit_workspace_bytes(size_t M, int K, int N, int x_bits) {
-    if (!sizes_ok(K, N) || (x_bits != 8 && x_bits != 32) || M >= (1u << 21) || few(M, x_bits == 8)) return 0;
+    if (!sizes_ok(K, N) || (x_bits != 8 && x_bits != 32) || M >= (1u << 21) || few(M, K, N, x_bits == 8)) return 0;
     const int splits = split_of((int)M, K, N).splits;
     return (size_t)up((int)M, BLOCK_ROWS) * (4 + (size_t)up(K, 128) * (x_bits == 8 ? 1 : 4)) + (splits > 1 ? (size_t)splits * M * up(N, 16) * 4 : 0);
 }
