@@ -202,6 +202,28 @@ def test_more_rows_than_one_launch_takes():
     assert np.all(np.abs(q.numpy() - want * (127 / most)[:, None]) <= 0.5 + 1e-9) and np.allclose(scale.numpy(), most / 127, rtol=2 * EPS)
 
 
+def test_rows_in_eight_bits_past_the_threads_of_one_launch_and_offsets_of_32_bits():
+    rng = np.random.default_rng(15)
+    rows, cols = (1 << 24) + 3, 257
+    gamma, row = (rng.standard_normal(cols).astype(np.float32) for _ in range(2))
+    x = be.zeros((rows, cols))
+    at = (0, 1 << 21, rows - 1)
+    for i in at:
+        x.leading(i, i + 1).set(row[None])
+    with xs.no_grad():
+        q, scale = F.rms_norm_8bit(xs.Tensor(x), _dev(gamma))
+    w = row.astype(np.float64)
+    want = w / np.sqrt((w * w).mean() + 1e-6) * gamma
+    most = np.abs(want).max()
+    scales = scale.numpy()
+    assert np.array_equal(np.flatnonzero(scales), at) and np.allclose(scales[list(at)], most / 127, rtol=2 * EPS, atol=0)
+    for i in at:
+        assert np.all(np.abs(q.eval.leading(i, i + 1).numpy()[0] - want * (127 / most)) <= 0.5 + 1e-9)
+    assert not q.eval.leading(rows - 3, rows - 1).numpy().any()
+    del x, q, scale
+    be.release_cached_memory()
+
+
 def test_only_the_scales_or_only_the_rows_want_a_gradient():
     rng = np.random.default_rng(11)
     x, r, gamma, dy, _ = _case(rng, 5, 70)

@@ -496,7 +496,7 @@ int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma
         const size_t n = a.rows;
         if (need <= 16) LAUNCH((rms_fwd_int8_kernel<16, 256, 1>), (n + 15) / 16, 256, a);
         else if (need <= 64) LAUNCH((rms_fwd_int8_kernel<64, 256, 1>), (n + 3) / 4, 256, a);
-        else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1>), rows, 256, a);
+        else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1>), n, 256, a);
         else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 1>), n, 1024, a);
         else if (need <= 4096) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 4>), n, 1024, a);
         else LAUNCH((rms_fwd_int8_long_kernel<1024>), n, 1024, a);
