@@ -157,6 +157,20 @@ def test_backward_in_one_pass_equals_that_in_steps(both):
         assert np.abs(a - b).max() <= 4 * 2 * EPS * max(1, np.abs(b).max())
 
 
+def test_a_gradient_of_the_sum_that_was_set_on_the_host():
+    rng = np.random.default_rng(16)
+    x, r, gamma, dy, ds = _case(rng, 5, 70)
+    grads = []
+    for place in (be.to_device, np.array):
+        tx, tr, tg = _dev(x, requires_grad=True), _dev(r, requires_grad=True), xs.Parameter(_dev(gamma, requires_grad=True))
+        y, s = F.rms_norm(tx, tg, tr)
+        s.grad = xs.Tensor(place(ds))
+        y.backward(_dev(dy))
+        grads.append([t.grad.numpy() for t in (tx, tr, tg)])
+        xs.GLOBAL.INPUTS = None
+    assert all(np.array_equal(a, b) for a, b in zip(*grads))
+
+
 def test_one_tensor_as_both_addends():
     rng = np.random.default_rng(10)
     x, _, gamma, dy, _ = _case(rng, 5, 70)

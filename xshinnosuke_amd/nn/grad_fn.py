@@ -371,7 +371,7 @@ def ResidualSumBackward(outputs):
             (second is None or (is_device(second) and (second._block is not first._block or
                                                        abs(first.address() - second.address()) >= first.nbytes)))):
         s = outputs.eval
-        K.rms_norm_bwd(dy, s, rstd, A.same_place(s, gamma.eval), None if outputs._grad is None else outputs.grad.eval, first, second, scale)
+        K.rms_norm_bwd(dy, s, rstd, A.same_place(s, gamma.eval), None if outputs._grad is None else A.same_place(s, outputs.grad.eval), first, second, scale)
         outputs._grad = None                         # it has never held the normalisation's part
     else:                                            # both addends one tensor, or gradients on the host
         _add_rms_norm_grad(outputs, gamma, dy, rstd)
