@@ -462,7 +462,7 @@ int xsmi_softmax_ce_bwd(const float *sm, const int64_t *labels, const float *ups
 /* ---- root-mean-square normalisation of rows ------------------------------------------------------------------
  * s = x + residual, r = 1 / sqrt(mean_j s_j^2 + eps), y_j = gamma_j s_j r over (rows, cols) float32 matrices, rows dense.  residual and sum
  * (the matrix s) come together or are both NULL (s = x); rstd (rows values r, or NULL) is what the backward
- * reads.  Sums are in float32: values of 1e19 and above overflow them.
+ * reads.  What is written may not overlap what is read.  Sums are in float32: values of 1e19 and above overflow them.
  * The int8 form stores q_j = round(127 y_j / max_i |y_i|), ties to even, and scale = max_i |y_i| / 127 for each row, with the sums and
  * the rounding in 64 bits; a row of zeros has the scale 0, one whose y are not all finite the numbers 0 and the scale NaN.
  * The reference normalises over the batch only (xs/layers/normalize.py:22-56). */
@@ -490,8 +490,8 @@ int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const 
  * writes the values (K, N) that they stand for.
  * xsmi_dense_4bit: y (M, N) = x (M, K) . weights (+ bias[N] or NULL).  x_scale NULL: x is float32; else x is int8 rows with
  * a float32 scale each, as xsmi_rms_norm_int8 writes them.  The workspace (needed for more rows than one
- * matrix instruction holds) is sized by the query, x_bits 32 or 8; M below 2^21.  The order of all sums depends on the
- * sizes alone.  The reference's dense layer is xs/nn/functional.py:99-120. */
+ * matrix instruction holds) is sized by the query, x_bits 32 or 8; M below 2^21.  y may not overlap what is read.  The
+ * order of all sums depends on the sizes alone.  The reference's dense layer is xs/nn/functional.py:99-120. */
 size_t xsmi_dense_4bit_code_bytes(int K, int N);
 size_t xsmi_dense_4bit_scale_count(int K, int N, int group);
 size_t xsmi_dense_4bit_workspace_bytes(size_t M, int K, int N, int x_bits);

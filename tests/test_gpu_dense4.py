@@ -204,6 +204,18 @@ def test_one_request_through_norm_and_packed_layers():
                 xs.GLOBAL.INPUTS = None
 
 
+def test_one_layer_twice_in_a_forward():
+    rng = np.random.default_rng(10)
+    weight, w = _weight(rng, 200, 200, 64)
+    layer, x = Dense4Bit(weight), rng.standard_normal((70, 200)).astype(np.float32)
+    with xs.no_grad():
+        first = layer(xs.Tensor(be.to_device(x)))
+        second = layer(first)
+        again = F.dense_4bit(first, weight)
+    assert first is not second and np.array_equal(second.numpy(), again.numpy())
+    assert np.all(np.abs(first.numpy() - x.astype(np.float64) @ w) <= _tolerance(x.astype(np.float64), w, 64))
+
+
 def values_of(weight):
     return weight.dequantize().numpy().astype(np.float64)
 
@@ -212,11 +224,12 @@ def test_refusals():
     rng = np.random.default_rng(9)
     weight, _ = _weight(rng, 64, 32, 32)
     x, q, s = be.to_device(np.ones((2, 64), np.float32)), be.to_device(np.ones((2, 64), np.int8)), be.to_device(np.ones(2, np.float32))
+    square, over = _weight(rng, 64, 64, 32)[0], be.zeros((4, 64))
     t = xs.Tensor
     with xs.no_grad():
         for call in (lambda: F.dense_4bit(t(q), weight), lambda: F.dense_4bit(t(x), weight, scale=t(s)), lambda: F.dense_4bit(t(x.reshape(4, 32)), weight),
                      lambda: F.dense_4bit(t(q), weight, scale=t(s.leading(0, 1))), lambda: F.dense_4bit(t(x), weight, t(s)),
-                     lambda: weight.product(x, out=be.empty((2, 31))), lambda: Weight4Bit(weight.codes, weight.scales, 64, 32, 64),
+                     lambda: weight.product(x, out=be.empty((2, 31))), lambda: square.product(over.leading(0, 2), out=over.leading(1, 3)), lambda: Weight4Bit(weight.codes, weight.scales, 64, 32, 64),
                      lambda: Weight4Bit(weight.codes, weight.scales, 64, 33, 32), lambda: Weight4Bit.quantize(x, 48), lambda: Weight4Bit.quantize(s, 32),
                      lambda: Weight4Bit.quantize(be.empty((0, 4)), 32), lambda: Dense4Bit.from_dense(Dense(3)), lambda: Dense4Bit(x)):
             with pytest.raises(ValueError):

@@ -96,9 +96,33 @@ def test_layer_in_both_graph_styles():
     assert all(p.grad is not None and np.abs(p.grad.eval).max() > 0 for p in net.parameters())
 
 
+def test_one_layer_twice_in_a_forward():
+    rng = np.random.default_rng(3)
+    x, w = xs.Tensor(rng.standard_normal((3, 4)), requires_grad=True), rng.standard_normal((3, 4))
+    norm = RMSNormalization(epsilon=0.1)
+
+    class Net(Module):
+        def forward(self, x):
+            a = norm(x)
+            return norm(a * xs.Tensor(w)) + a
+
+    Net()(x).backward(xs.Tensor(np.ones((3, 4))))
+    grads = [t.grad.eval.copy() for t in (x, norm.parameters()[0])]
+    xs.GLOBAL.INPUTS = None
+    u, gamma = xs.Tensor(x.eval.copy(), requires_grad=True), xs.Parameter(xs.Tensor(np.ones(4), requires_grad=True))
+    a = F.rms_norm(u, gamma, epsilon=0.1)
+    z = F.rms_norm(a * xs.Tensor(w), gamma, epsilon=0.1) + a
+    z.backward(xs.Tensor(np.ones((3, 4))))
+    for got, want in zip(grads, (u.grad.eval, gamma.grad.eval)):
+        np.testing.assert_allclose(got, want, rtol=1e-6, atol=1e-7)       # the layer's scales are float32
+
+
 def test_refusals():
     rng = np.random.default_rng(2)
     x, r, gamma = _tensors(rng, (3, 4))
+    for out in (x, r, gamma):
+        with pytest.raises(ValueError):
+            F.rms_norm(x, gamma, r, out=out)
     with pytest.raises(ValueError):
         F.rms_norm(x, xs.Parameter(xs.Tensor(np.ones(3))))
     with pytest.raises(ValueError):

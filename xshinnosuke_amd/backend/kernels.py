@@ -852,6 +852,10 @@ def full(shape, value):
 _F32, _I8 = np.dtype(np.float32), np.dtype(np.int8)
 
 
+def _overlaps(out, *arrays):
+    return any(a is not None and a._block is out._block and out._offset < a._offset + a.nbytes and a._offset < out._offset + out.nbytes for a in arrays)
+
+
 def _rms_operands(x, gamma, residual):
     shape = x.shape
     if x.dtype != _F32 or gamma.dtype != _F32 or (residual is not None and residual.dtype != _F32):
@@ -870,6 +874,8 @@ def rms_norm_fwd(x, gamma, eps, residual=None, y=None, want_rstd=True):
     if y is None:
         y = _array.empty_like(x)
     else:
+        if _overlaps(y, x, gamma, residual):
+            raise ValueError("rms_norm: the output lies over an operand")
         _like(x, y).take_fresh()
     rstd = empty((rows,)) if want_rstd else None
     if residual is None:
@@ -968,6 +974,8 @@ def dense_4bit(x, codes, scales, inputs, outputs, group, bias=None, x_scale=None
         out = DeviceArray(shape[:-1] + (outputs,), _F32)
     elif out.size != rows * outputs or out.dtype != _F32:
         raise ValueError("dense_4bit: output has shape %s, expected %s" % (out.shape, shape[:-1] + (outputs,)))
+    elif _overlaps(out, x, bias, x_scale):
+        raise ValueError("dense_4bit: the output lies over an operand")
     else:
         out.take_fresh()
     key = ("dense4", rows, inputs, outputs, x_scale is None)

@@ -84,7 +84,7 @@ class Dense4Bit(FusedActivation, Layer):
         self._static_act_buffer()
 
     def call(self, x, scale=None, *args, **kwargs):
-        out = self._data
+        out = None if x.is_dynamic else self._data       # a dynamic call may read what the one before it wrote
         if out is not None and (out.eval is None or tuple(out.shape) != tuple(x.shape[:-1]) + (self.out_features,)):
             out = None
         self._data = F.dense_4bit(x, self.weight, self.bias, scale, out)

@@ -49,7 +49,7 @@ class RMSNormalization(Layer):
         self._parameters.append(Parameter(self.gamma_initializer(self._input_shape[-1], requires_grad=True)))
 
     def call(self, x, residual=None, *args, **kwargs):
-        out = self._data
+        out = None if x.is_dynamic else self._data       # a dynamic call may be the second of a forward: its output is its own
         if out is not None and out.eval is not None and tuple(out.shape) != tuple(x.shape):
             out = None
         y = F.rms_norm(x, self._parameters[0], residual, self.epsilon, out)

@@ -520,6 +520,8 @@ def rms_norm(inputs, gamma, residual=None, epsilon=1e-6, out=None):
     _mark_input(inputs)
     if not epsilon >= 0:
         raise ValueError('rms_norm: epsilon must not be negative')
+    if out is not None and any(out is t for t in (inputs, residual, gamma)):
+        raise ValueError('rms_norm: out must not be one of the operands')
     dst = None if out is None else out.eval
     y, s, rstd = A.rms_norm(inputs.eval, gamma.eval, epsilon, None if residual is None else residual.eval, dst)
     if out is None:
