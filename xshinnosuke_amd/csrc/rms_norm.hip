@@ -87,6 +87,7 @@ struct Forward {
 };
 
 // T threads a row, NT threads a workgroup, V vectors of four a thread: rows of up to 4 T V elements stay in registers.
+// 16384 x 4096 with a residual: 174 us, 6.2 TB/s; 32 x 512: 2.9 us, a chain of load, sum across the workgroup and store.
 template <int T, int NT, int V, bool STREAM>
 __global__ void __launch_bounds__(NT) rms_fwd_kernel(Forward a) {
     __shared__ float sm[NT / 64];
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(NT) rms_fwd_kernel(Forward a) {
     }
 }
 
-// Longer rows: a workgroup reads its row twice.
+// Longer rows: a workgroup reads its row twice (512 x 65536 with a residual: 125 us, 81 for the bytes).
 template <int NT>
 __global__ void __launch_bounds__(NT) rms_fwd_long_kernel(Forward a) {
     __shared__ float sm[NT / 64];
@@ -162,7 +163,7 @@ __device__ __forceinline__ void store_q(int8_t *p, int j, int cols, const double
 // The output in 8 bits: q_j = round(127 y_j / max |y|), scale = max |y| / 127.  The root is common to a row's y, so the numbers are those of
 // z_j = gamma_j s_j, and the sum and the largest value are found together.  In 64 bits, which run at the rate of 32 here and
 // are not what bounds this: a number next to a border falls on the side that the exact value is on, whatever the order
-// of the sums.  A row of zeros has the numbers 0 and the scale 0, one with a NaN or an infinity the numbers 0 and the scale NaN.
+// of the sums.  16384 x 4096 with a residual: 137 us, 6.4 TB/s; one row of 4096: 4.9 us.  A row of zeros has the numbers 0 and the scale 0, one with a NaN or an infinity the numbers 0 and the scale NaN.
 struct Steps {
     bool bad;
     double inverse;
@@ -173,7 +174,7 @@ __device__ __forceinline__ Steps steps_of(const Forward &a, double sq, double mo
     return Steps{bad, bad || most == 0.0 ? 0.0 : 127.0 / most};
 }
 
-template <int T, int NT, int V>
+template <int T, int NT, int V, bool STREAM>
 __global__ void __launch_bounds__(NT) rms_fwd_int8_kernel(Forward a) {
     __shared__ double2 sm[NT / 64];
     const uint64_t row = (uint64_t)blockIdx.x * (NT / T) + threadIdx.x / T;
@@ -186,9 +187,9 @@ __global__ void __launch_bounds__(NT) rms_fwd_int8_kernel(Forward a) {
         const int j = 4 * (v * T + t);
         s[v] = g[v] = f4{0.f, 0.f, 0.f, 0.f};
         if (live && j < cols) {
-            s[v] = load4(a.x + at, j, cols);
+            s[v] = load4<STREAM>(a.x + at, j, cols);
             g[v] = load4(a.gamma, j, cols);
-            if (a.residual) s[v] += load4(a.residual + at, j, cols);
+            if (a.residual) s[v] += load4<STREAM>(a.residual + at, j, cols);
         }
     }
     double sq = 0.0, most = 0.0;
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(NT) rms_fwd_int8_kernel(Forward a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int j = 4 * (v * T + t);
-        if (a.sum && live && j < cols) store4(a.sum + at, j, cols, s[v]);
+        if (a.sum && live && j < cols) store4<STREAM>(a.sum + at, j, cols, s[v]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const double z = (double)s[v][e] * (double)g[v][e];
@@ -286,8 +287,9 @@ __device__ __forceinline__ void rms_columns(const Backward &a, int block) {
 }
 
 // T threads a row; a workgroup takes every (NT / T gridDim)-th lot of rows, and adds the terms of dgamma of the columns
-// that a thread owns in its registers; they go to part[group of rows] at the end.  All that a row needs is loaded before its sum is
-// formed.
+// that a thread owns in its registers; those of a workgroup go to its row of part at the end.  All that a row needs is loaded before its sum is
+// formed.  16384 x 4096 with ds and two gradients: 224 us, 6.0 TB/s, and 5 for the sums of part.  Rows that a workgroup has side by
+// side share its row of part: with one for each of them 65536 x 33 took 62 us instead of 16, for the one workgroup that adds 16384.
 template <int T, int NT, int V, bool STREAM>
 __global__ void __launch_bounds__(NT) rms_bwd_kernel(Backward a) {
     __shared__ float sm[NT / 64];
@@ -342,7 +344,26 @@ __global__ void __launch_bounds__(NT) rms_bwd_kernel(Backward a) {
         }
     }
     if (a.part) {
-        float *part = a.part + ((uint64_t)blockIdx.x * (NT / T) + threadIdx.x / T) * (uint64_t)cols;
+        if (T < NT) {                                // the rows that were worked on side by side
+            constexpr int W = NT / 64, L = T < 64 ? T : 64;
+            __shared__ f4 beside[W][V][L];
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int o = 32; o >= T; o >>= 1)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dg[v][e] += __shfl_xor(dg[v][e], o);
+            if ((threadIdx.x & 63) < L)
+#pragma unroll
+                for (int v = 0; v < V; ++v) beside[threadIdx.x >> 6][v][t] = dg[v];
+            __syncthreads();
+            if (threadIdx.x >= T) return;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int w = 1; w < W; ++w) dg[v] += beside[w][v][t];
+        }
+        float *part = a.part + (uint64_t)blockIdx.x * cols;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int j = 4 * (v * T + t);
@@ -351,7 +372,8 @@ __global__ void __launch_bounds__(NT) rms_bwd_kernel(Backward a) {
     }
 }
 
-// Longer rows, read twice; the terms of dgamma are added in memory, in this workgroup's own row of part.
+// Longer rows, read twice; the terms of dgamma are added in memory, in this workgroup's own row of part (512 x 65536: 185 us, 81 for
+// the bytes without part).
 template <int NT>
 __global__ void __launch_bounds__(NT) rms_bwd_long_kernel(Backward a) {
     __shared__ float sm[NT / 64];
@@ -380,7 +402,7 @@ __global__ void __launch_bounds__(NT) rms_bwd_long_kernel(Backward a) {
 }
 
 // dgamma[j] = (accumulate ? dgamma[j] : 0) + sum over the rows of part: 32 columns a workgroup, eight threads of four columns for each
-// of 128 stretches of rows.
+// of 128 stretches of rows (512 rows of 4096: 5.0 us, most of it the launch and the joining).
 __global__ void __launch_bounds__(1024) rms_dgamma_kernel(const float *__restrict__ part, int rows, int cols, float *dgamma, int accumulate) {
     __shared__ f4 sm[128][8];
     const int t = threadIdx.x & 7, j = blockIdx.x * 32 + 4 * t, w = threadIdx.x >> 3;
@@ -418,21 +440,20 @@ Forward lot(Forward a, size_t first) {
     return a;
 }
 
-// Workgroups of the backward, and the rows of part that they write.
-struct BackwardPlan {
-    int threads_a_row, threads, groups, parts;
-};
-BackwardPlan backward_plan(uint64_t rows, int cols) {
-    BackwardPlan p;
-    const int need = (cols + 3) / 4;
-    p.threads_a_row = need <= 16 ? 16 : need <= 64 ? 64 : need <= 256 ? 256 : 1024;
-    p.threads = p.threads_a_row == 1024 ? 1024 : 256;
-    const uint64_t lots = (rows + p.threads / p.threads_a_row - 1) / (p.threads / p.threads_a_row);
+// Many rows go by a wave each up to 1024 columns, without a barrier (65536 x 257, backward: 80 us, by workgroups of 256 threads 123), and
+// in 8 bits by narrower workgroups above (16384 x 4096: 137 us, by 1024 threads 252; 13000 x 5000: 158 and 246); few rows go by as
+// many threads as they have use for (200 x 1000, backward: 3.8 us, by waves 4.2).  The forward of more than 512 columns goes by
+// waves only where the operands stay in the caches (2048 x 600: 6.9 us, by workgroups 9.1; 65536 x 600: 123 and 113).
+constexpr uint64_t WAVE_ROWS = 512;
+inline bool by_waves(uint64_t rows) { return rows >= WAVE_ROWS; }
+
+// Workgroups of the backward, each with a row of part.
+int backward_groups(uint64_t rows, int cols) {
+    const int need = (cols + 3) / 4, side = need <= 16 ? 16 : need <= 64 || (need <= 256 && by_waves(rows)) ? 4 : 1;       // rows side by side
+    const uint64_t lots = (rows + side - 1) / side;
     // as many workgroups as fill the card, and at least two lots of rows each where there are more than two a compute unit
     const uint64_t most = need > 1024 ? 256 : 1024, few = most / 2, two = (lots + 1) / 2;
-    p.groups = (int)(lots <= few ? lots : two <= few ? few : two < most ? two : most);
-    p.parts = p.groups * (p.threads / p.threads_a_row);
-    return p;
+    return (int)(lots <= few ? lots : two <= few ? few : two < most ? two : most);
 }
 
 // Few rows: dgamma by workgroups of its own, which read dy and s again beside the ones of the rows, in one launch and without a
@@ -475,6 +496,8 @@ int xsmi_rms_norm_fwd(const float *x, const float *residual, const float *gamma,
         const size_t n = a.rows;
         if (need <= 16) LAUNCH_TWO(rms_fwd_kernel, 16, 256, 1, (n + 15) / 16, a);
         else if (need <= 64) LAUNCH_TWO(rms_fwd_kernel, 64, 256, 1, (n + 3) / 4, a);
+        else if (need <= 128 && by_waves(n)) LAUNCH_TWO(rms_fwd_kernel, 64, 256, 2, (n + 3) / 4, a);
+        else if (need <= 256 && by_waves(n) && !stream) LAUNCH((rms_fwd_kernel<64, 256, 4, false>), (n + 3) / 4, 256, a);
         else if (need <= 256) LAUNCH_TWO(rms_fwd_kernel, 256, 256, 1, n, a);
         else if (need <= 1024) LAUNCH_TWO(rms_fwd_kernel, 512, 512, 2, n, a);
         else if (need <= 4096) LAUNCH_TWO(rms_fwd_kernel, 1024, 1024, 4, n, a);
@@ -490,15 +513,20 @@ int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma
     if (int rc = check("xsmi_rms_norm_int8", rows, cols, eps)) return rc;
     if (rows == 0) return XSMI_OK;
     XSMI_CHECK_ARG(x && gamma && q && scale && (residual == nullptr) == (sum == nullptr), "xsmi_rms_norm_int8: null pointer (a residual comes with a sum)");
+    const bool stream = streams(rows, cols, residual ? 3 : 1);
     const int need = (cols + 3) / 4;
     for (size_t first = 0; first < rows; first += LAUNCH_ROWS) {
         const Forward a = lot({x, residual, gamma, sum, nullptr, nullptr, q, scale, rows, cols, eps}, first);
         const size_t n = a.rows;
-        if (need <= 16) LAUNCH((rms_fwd_int8_kernel<16, 256, 1>), (n + 15) / 16, 256, a);
-        else if (need <= 64) LAUNCH((rms_fwd_int8_kernel<64, 256, 1>), (n + 3) / 4, 256, a);
-        else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1>), n, 256, a);
-        else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 1>), n, 1024, a);
-        else if (need <= 4096) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 4>), n, 1024, a);
+        if (need <= 16) LAUNCH_TWO(rms_fwd_int8_kernel, 16, 256, 1, (n + 15) / 16, a);
+        else if (need <= 64) LAUNCH_TWO(rms_fwd_int8_kernel, 64, 256, 1, (n + 3) / 4, a);
+        else if (need <= 128 && by_waves(n)) LAUNCH_TWO(rms_fwd_int8_kernel, 64, 256, 2, (n + 3) / 4, a);
+        else if (need <= 256 && by_waves(n)) LAUNCH_TWO(rms_fwd_int8_kernel, 64, 256, 4, (n + 3) / 4, a);
+        else if (need <= 256) LAUNCH((rms_fwd_int8_kernel<256, 256, 1, false>), n, 256, a);
+        else if (need <= 1024 && by_waves(n)) LAUNCH_TWO(rms_fwd_int8_kernel, 256, 256, 4, n, a);
+        else if (need <= 1024) LAUNCH((rms_fwd_int8_kernel<1024, 1024, 1, false>), n, 1024, a);
+        else if (need <= 2048 && by_waves(n)) LAUNCH_TWO(rms_fwd_int8_kernel, 512, 512, 4, n, a);
+        else if (need <= 4096) LAUNCH_TWO(rms_fwd_int8_kernel, 1024, 1024, 4, n, a);
         else LAUNCH((rms_fwd_int8_long_kernel<1024>), n, 1024, a);
         XSMI_LAUNCH_CHECK("rms_fwd_int8_kernel");
     }
@@ -507,7 +535,7 @@ int xsmi_rms_norm_int8(const float *x, const float *residual, const float *gamma
 
 size_t xsmi_rms_norm_workspace_bytes(size_t rows, int cols) {
     if (rows == 0 || rows >= MAX_ROWS || cols < 1 || cols > (1 << 30) || columns_apart(rows, cols)) return 0;
-    return (size_t)backward_plan(rows, cols).parts * (size_t)cols * sizeof(float);
+    return (size_t)backward_groups(rows, cols) * (size_t)cols * sizeof(float);
 }
 
 int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const float *gamma, const float *ds, float *dx1, float beta1,
@@ -522,22 +550,24 @@ int xsmi_rms_norm_bwd(const float *dy, const float *s, const float *rstd, const 
     const size_t want = dgamma ? xsmi_rms_norm_workspace_bytes(rows, cols) : 0;
     XSMI_CHECK_ARG(ws_bytes >= want && (ws || !want) && ((uintptr_t)ws & 15) == 0, "xsmi_rms_norm_bwd: workspace of %zu bytes, needs %zu", ws_bytes, want);
     if (!dx1 && !dgamma) return XSMI_OK;
-    const BackwardPlan p = backward_plan(rows, cols);
+    const int groups = backward_groups(rows, cols);
     const bool apart = dgamma && columns_apart(rows, cols);
     const Backward a = {dy, s, rstd, gamma, ds, dx1, dx2, dgamma && !apart ? (float *)ws : nullptr, beta1 != 0.f, beta2 != 0.f, rows, cols,
-                        apart ? dgamma : nullptr, beta_gamma != 0.f, p.groups};
-    const int grid = p.groups + (apart ? (cols + 31) / 32 : 0);
+                        apart ? dgamma : nullptr, beta_gamma != 0.f, groups};
+    const int grid = groups + (apart ? (cols + 31) / 32 : 0);
     const bool stream = streams(rows, cols, 3 + (ds != nullptr) + (dx2 != nullptr));
     const int need = (cols + 3) / 4;
     if (need <= 16) LAUNCH_TWO(rms_bwd_kernel, 16, 256, 1, grid, a);
     else if (need <= 64) LAUNCH_TWO(rms_bwd_kernel, 64, 256, 1, grid, a);
-    else if (need <= 256) LAUNCH_TWO(rms_bwd_kernel, 256, 256, 1, grid, a);
+    else if (need <= 128 && by_waves(rows)) LAUNCH_TWO(rms_bwd_kernel, 64, 256, 2, grid, a);
+    else if (need <= 256 && by_waves(rows)) LAUNCH_TWO(rms_bwd_kernel, 64, 256, 4, grid, a);
+    else if (need <= 256) LAUNCH((rms_bwd_kernel<256, 256, 1, false>), grid, 256, a);
     else if (need <= 1024) LAUNCH_TWO(rms_bwd_kernel, 1024, 1024, 1, grid, a);
     else if (need <= 4096) LAUNCH_TWO(rms_bwd_kernel, 1024, 1024, 4, grid, a);
-    else LAUNCH((rms_bwd_long_kernel<1024>), p.groups, 1024, a);
+    else LAUNCH((rms_bwd_long_kernel<1024>), groups, 1024, a);
     XSMI_LAUNCH_CHECK("rms_bwd_kernel");
     if (dgamma && !apart) {
-        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((cols + 31) / 32), dim3(1024), 0, xsmi::stream(), (const float *)ws, p.parts, cols, dgamma,
+        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((cols + 31) / 32), dim3(1024), 0, xsmi::stream(), (const float *)ws, groups, cols, dgamma,
                            beta_gamma != 0.f);
         XSMI_LAUNCH_CHECK("rms_dgamma_kernel");
     }
