@@ -623,44 +623,55 @@ __global__ void __launch_bounds__(256) dense4_join_kernel(Dense a, const float *
 }
 
 // ---- the weights -------------------------------------------------------------------------------------------------
-// One thread for a lane's eight inputs of a step, one output: a group's value of largest magnitude becomes -8, whatever its
-// sign, and the others go to the nearest number.  The value is looked for by every thread of its group again.
+// One workgroup for a tile's 1 KB of a chunk, one thread for eight inputs of an output: a group's value of largest magnitude becomes -8,
+// whatever its sign, and the others go to the nearest number.  8192 x 8192: 95 us, 3.2 TB/s (976 where every thread went through its
+// group by itself).
+__device__ __forceinline__ float farther(float a, float b) {         // the first of equals; a NaN stays
+    return a != a || fabsf(b) <= fabsf(a) ? a : b;
+}
 __global__ void __launch_bounds__(256) quantize4_kernel(const float *__restrict__ w, uint8_t *codes, _Float16 *scales, int K, int N, int group, int chunks, int cols) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x, total = (uint64_t)(cols / 16) * chunks * 256;
-    if (i >= total) return;
-    const int j = (int)(i & 3), lane = (int)(i >> 2) & 63;
-    const uint64_t tc = i >> 8;
-    const int c = (int)(tc % (uint64_t)chunks), t = (int)(tc / (uint64_t)chunks);
-    const int n = t * 16 + (lane & 15), k0 = c * 128 + j * 32 + (lane >> 4) * 8, g = k0 / group;
+    __shared__ float far[16][17];                    // [octet of inputs][output]
+    const int c = (int)(blockIdx.x % (uint32_t)chunks), t = (int)(blockIdx.x / (uint32_t)chunks);
+    const int in = threadIdx.x & 15, o = threadIdx.x >> 4, n = t * 16 + in, k0 = c * 128 + o * 8;
+    float v[8], most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = n < N && k0 + e < K ? w[(uint64_t)(k0 + e) * N + n] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = farther(most, v[e]);
+    far[o][in] = most;
+    __syncthreads();
+    const int octets = group / 8, first = o / octets * octets;
     float extreme = 0.f;
-    if (n < N)
-        for (int k = g * group; k < min(K, (g + 1) * group); ++k) {
-            const float v = w[(uint64_t)k * N + n];
-            if (!(fabsf(v) <= fabsf(extreme))) extreme = v;          // the first of equals; a NaN stays
-            if (extreme != extreme) break;
-        }
+    for (int i = first; i < first + octets; ++i) extreme = farther(extreme, far[i][in]);
     const _Float16 s = (_Float16)(extreme / -8.f);
     const float sf = (float)s;
     uint32_t word = 0;
+#pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int k = k0 + e;
-        const float v = n < N && k < K ? w[(uint64_t)k * N + n] : 0.f;
-        const float r = sf == 0.f || v == 0.f ? 0.f : fminf(fmaxf(rintf(v / sf), -8.f), 7.f);
+        const float r = sf == 0.f || v[e] == 0.f ? 0.f : fminf(fmaxf(rintf(v[e] / sf), -8.f), 7.f);
         word |= ((uint32_t)(int)r & 15u) << (4 * e);
     }
-    reinterpret_cast<uint32_t *>(codes)[(tc * 64 + lane) * 4 + j] = word;
-    if (k0 % group == 0) scales[(uint64_t)g * cols + n] = s;
+    // octet o is step o / 4 of lanes 16 (o % 4) and on
+    reinterpret_cast<uint32_t *>(codes)[((uint64_t)blockIdx.x * 64 + 16 * (o & 3) + in) * 4 + (o >> 2)] = word;
+    if (o == first) scales[(uint64_t)((k0 - c * 128) / group + c * (128 / group)) * cols + n] = s;
 }
 
+// One workgroup for four tiles of a chunk, a wave for each, a lane for the 32 inputs of an output that lie together.
+// 8192 x 8192: 70 us, 4.3 TB/s (a thread for each weight: 158).
 __global__ void __launch_bounds__(256) dequantize4_kernel(const uint8_t *__restrict__ codes, const _Float16 *__restrict__ scales, float *w, int K, int N, int group,
                                                           int chunks, int cols) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (uint64_t)K * N) return;
-    const int k = (int)(i / (uint64_t)N), n = (int)(i - (uint64_t)k * N), r = k & 127;
-    const uint64_t tile = (uint64_t)(n >> 4) * chunks + (k >> 7);
-    const uint8_t b = codes[(tile * 64 + 16 * (r % 32 / 8) + (n & 15)) * 16 + 4 * (r / 32) + r % 8 / 2];
-    const int c = (int)((k & 1 ? b >> 4 : b & 15) ^ 8) - 8;
-    w[i] = (float)c * (float)scales[(uint64_t)(k / group) * cols + n];
+    const int c = (int)(blockIdx.x % (uint32_t)chunks), t = (int)(blockIdx.x / (uint32_t)chunks) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, n = t * 16 + (lane & 15);
+    if (n >= N) return;
+    const u4 x = reinterpret_cast<const u4 *>(codes)[((uint64_t)t * chunks + c) * 64 + lane];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int k0 = c * 128 + 32 * j + 8 * (lane >> 4);
+        const float s = (float)scales[(uint64_t)(c * (128 / group) + 32 * j / group) * cols + n];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (k0 + e < K) w[(uint64_t)(k0 + e) * N + n] = (float)((int)((x[j] >> (4 * e) & 15u) ^ 8u) - 8) * s;
+    }
 }
 
 inline int up(int v, int to) { return (v + to - 1) / to * to; }
@@ -789,9 +800,10 @@ int xsmi_dequantize_4bit(const uint8_t *codes, const void *scales, int K, int N,
     XSMI_REQUIRE_INIT();
     if (int rc = check_weights("xsmi_dequantize_4bit", K, N, group)) return rc;
     XSMI_CHECK_ARG(w && codes && scales, "xsmi_dequantize_4bit: null pointer");
-    const uint64_t groups = ((uint64_t)K * N + 255) / 256;
+    const int chunks = up(K, 128) / 128;
+    const uint64_t groups = (uint64_t)((up(N, 16) / 16 + 3) / 4) * chunks;
     XSMI_CHECK_ARG(groups < (1u << 24), "xsmi_dequantize_4bit: %d x %d weights", K, N);
-    hipLaunchKernelGGL(dequantize4_kernel, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), codes, (const _Float16 *)scales, w, K, N, group, up(K, 128) / 128, up(N, 16));
+    hipLaunchKernelGGL(dequantize4_kernel, dim3((uint32_t)groups), dim3(256), 0, xsmi::stream(), codes, (const _Float16 *)scales, w, K, N, group, chunks, up(N, 16));
     XSMI_LAUNCH_CHECK("dequantize4_kernel");
     return XSMI_OK;
 }
