@@ -67,6 +67,12 @@ def test_products(k, n, group):
         assert np.all(np.abs(y - (x @ w + more)) <= _tolerance(x, w, group, True) + EPS * np.abs(more)), m
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("k,n", [(1500, 4100), (3000, 4130), (5000, 4150)])
+def test_products_of_more_tiles_than_compute_units(k, n, group):
+    test_products(k, n, group)
+
+
 @pytest.mark.parametrize("m", [1, 3, 8, 40])
 def test_rows_are_their_own(m):
     """Rows of very different sizes, zeros, the largest and smallest values, infinities and NaN: none changes another row."""

@@ -130,14 +130,19 @@ __device__ __forceinline__ void digits8(const int *x, u2 *to) {
 
 // DIGITS 1: int8 rows, 4: float32 rows; CT tiles of 16 columns (a row and digit each), of which RPT octets a thread lays out.
 // Columns without a row repeat the last one: a column's sums are its own.  LOOP: there is more than one window.
-template <int G, int DIGITS, int CT, int NT, int PF, int RPT, bool LOOP>
+// One row, 8192 x 8192, groups of 128: 9.5 us, 3.6 TB/s, a chain of loads, digits, sums and their join; what a wave does between loads is
+// longer than the loads.  SIDE: where rows are so few that all groups of a chunk find columns side by side, each column meets zeros outside of its group, and
+// a chunk's sums are scaled once and not once for each group (one row, 8192 x 16384, groups of 32: 28.7 -> 21.6 us; 8-bit: 26.1 -> 18.2).
+template <int G, int DIGITS, int CT, int NT, int PF, int RPT, bool LOOP, bool SIDE>
 __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int unusual[16];
-    constexpr int GROUPS = 128 / G;                  // of a chunk
+    constexpr int GROUPS = 128 / G, SCALES = SIDE ? 1 : GROUPS;      // of a chunk, and those whose scales a lane needs
     constexpr bool F32 = DIGITS == 4;
+    static_assert(!SIDE || (CT == 1 && GROUPS > 1), "groups side by side share one tile of columns");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, col = lane & 15;
-    const int M = a.M, R = M * DIGITS, tiles = a.cols / 16, t0 = blockIdx.x * NT;
+    const int M = a.M, R = M * DIGITS, own = SIDE ? min(col / R, GROUPS - 1) : 0;      // the group of this lane's column
+    const int tiles = a.cols / 16, t0 = blockIdx.x * NT;
     if (F32 && threadIdx.x < 16) unusual[threadIdx.x] = 0;
     if (F32) __syncthreads();
     // A row's part of a window, 16 PF octets, is laid out by `share` lanes (float32: one row of a lane's own, so that the
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
     float xf[F32 ? RPT : 1][8];
     i2 xi[F32 ? 1 : RPT];
     u4 w[NT][PF];
-    h4 s[NT][PF][GROUPS];
+    h4 s[NT][PF][SCALES];
     // the octet of this thread's i-th in a window: row, chunk of the window, octet of the chunk
     auto place = [&](int i, int &r, int &k, int &o) {
         if (F32) {
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
                 const int c = min(c0 + i * WAVES, chunks - 1);       // a repeated chunk meets rows of zeros
                 w[t][i] = codes[(uint64_t)c * 64];
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) s[t][i][g] = *reinterpret_cast<const h4 *>(a.scales + (uint64_t)(c * GROUPS + g) * a.cols + tile * 16 + 4 * q);
+                for (int g = 0; g < SCALES; ++g) s[t][i][g] = *reinterpret_cast<const h4 *>(a.scales + (uint64_t)(c * GROUPS + own + g) * a.cols + tile * 16 + 4 * q);
             }
         }
     };
@@ -236,14 +241,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
             }
         }
         u4 wc[NT][PF];
-        h4 sc[NT][PF][GROUPS];
+        h4 sc[NT][PF][SCALES];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < PF; ++i) {
                 wc[t][i] = w[t][i];
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) sc[t][i][g] = s[t][i][g];
+                for (int g = 0; g < SCALES; ++g) sc[t][i][g] = s[t][i][g];
             }
         if (LOOP && c0 + WAVES * PF < chunks) load(c0 + WAVES * PF);
         asm volatile("" ::: "memory");               // a wave's LDS operations stay in order
@@ -256,30 +261,36 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
         for (int i = 0; i < PF; ++i) {
 #pragma unroll
             for (int u = 0; u < CT; ++u) {
-                const int row = min(u * 16 + col, R - 1);
+                const int row = min(u * 16 + col - own * R, R - 1);
                 i4 x[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) x[j] = reinterpret_cast<const i4 *>(mine)[((i * 2 + j) * 4 + q) * R + row];
+                for (int j = 0; j < 2; ++j) {
+                    x[j] = reinterpret_cast<const i4 *>(mine)[((i * 2 + j) * 4 + q) * R + row];
+                    if (SIDE) {                      // inputs 64 j and on, of which the second half may be of another group
+                        const int lo = own == 2 * j * 32 / G ? -1 : 0, hi = own == (2 * j + 1) * 32 / G ? -1 : 0;
+                        x[j].x &= lo, x[j].y &= lo, x[j].z &= hi, x[j].w &= hi;
+                    }
+                }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     i4 d = {0, 0, 0, 0};
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const u2 lo = weights_i8(wc[t][i][2 * j]), hi = weights_i8(wc[t][i][2 * j + 1]);
-                        if (G == 32) {
+                        if (G == 32 && !SIDE) {
                             const i4 zero = {0, 0, 0, 0};
                             const i4 e = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, lo), __builtin_bit_cast(long, i2{x[j].x, x[j].y}), zero, 0, 0, 0);
                             const i4 f = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, hi), __builtin_bit_cast(long, i2{x[j].z, x[j].w}), zero, 0, 0, 0);
 #pragma unroll
                             for (int v = 0; v < 4; ++v) {
-                                sum[t][u][v] += (float)sc[t][i][2 * j][v] * (float)e[v];
-                                sum[t][u][v] += (float)sc[t][i][2 * j + 1][v] * (float)f[v];
+                                sum[t][u][v] += (float)sc[t][i][2 * j % SCALES][v] * (float)e[v];
+                                sum[t][u][v] += (float)sc[t][i][(2 * j + 1) % SCALES][v] * (float)f[v];
                             }
                         } else {
                             d = __builtin_amdgcn_mfma_i32_16x16x64_i8(i4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y}, x[j], d, 0, 0, 0);
-                            if (G == 64 || j == 1) {
+                            if ((G == 64 && !SIDE) || j == 1) {
 #pragma unroll
-                                for (int v = 0; v < 4; ++v) sum[t][u][v] += (float)sc[t][i][G == 64 ? j : 0][v] * (float)d[v];
+                                for (int v = 0; v < 4; ++v) sum[t][u][v] += (float)sc[t][i][j % SCALES][v] * (float)d[v];
                                 d = i4{0, 0, 0, 0};
                             }
                         }
@@ -291,7 +302,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
 #pragma unroll
         for (int u = 0; u < CT; ++u) {
             // a column's digit, the sixteen in its weights, and its row's power of two in this wave and window
-            const int row = min(u * 16 + col, R - 1);
+            const int row = min(u * 16 + col - own * R, R - 1);
             const int e = F32 ? __shfl(exponent, row / 4 * share) + 8 * (row & 3) - 4 : -4;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -312,7 +323,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
         float y = 0.f;
         for (int k = 0; k < WAVES; ++k)
 #pragma unroll
-            for (int e = DIGITS - 1; e >= 0; --e) y += part[((k * NT + t) * CT * 16 + r * DIGITS + e) * 16 + (i & 15)];
+            for (int e = DIGITS - 1; e >= 0; --e)
+                for (int g = 0; g < (SIDE ? GROUPS : 1); ++g) y += part[((k * NT + t) * CT * 16 + g * R + r * DIGITS + e) * 16 + (i & 15)];
         if (!F32) y *= a.x_scale[r];
         if (F32 && unusual[r]) {                     // what is not finite decides; one thread goes through the row
             const float *const x = static_cast<const float *>(a.x) + (uint64_t)r * a.K;
@@ -330,7 +342,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
 // ---- many rows ---------------------------------------------------------------------------------------------------
 // The rows are laid out first as the matrix instructions read them, for each 64 rows and chunk of 128 inputs in one piece:
 // float32 [step of 32 inputs][tile of 16 rows][part][lane], a lane's octet of one row as float16; int8 [64 inputs][tile][lane][octets o and o + 4].
-// One workgroup a row.  Rows behind the last one are not written: a column's sums are its own.
+// One workgroup a row (200 x 4096: 7.3 us, 3.8 without its stores).  Rows behind the last one are not written: a column's sums are its own.
 constexpr int BLOCK_ROWS = 64;
 constexpr uint32_t piece_bytes(bool int8) { return int8 ? 64 * 128 : 64 * 128 * 4; }
 constexpr int many_stages(bool int8) { return int8 ? 4 : 2; }
@@ -386,7 +398,9 @@ __global__ void __launch_bounds__(256) dense4_rows_kernel(Dense a, char *operand
 // Each weight is turned into float16 by one wave only, for 64 rows: where two waves do it for 32 rows each, that takes
 // the vector unit as long as the multiplications take the matrix unit.  float32 rows fill the LDS with two stages, and a wave loads its codes
 // and scales into registers; 8-bit rows, which are multiplied faster than a load comes back, leave room for four stages with
-// codes and scales.
+// codes and scales.  200 rows, 4096 x 8192, groups of 128: 36.8 us, 730 TFLOP/s of two-part multiplications; 8-bit rows 20 us.  A
+// pair of chunks takes 1.85 us, of which the matrix unit is busy for 0.96; without its loads 1.6, without its barrier 1.6, without
+// reading the rows 1.7: nothing alone bounds it.
 template <int G, bool INT8>
 __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char *operand, const float *back, float *part, int each) {
     constexpr uint32_t ROWS = piece_bytes(INT8), STAGE = many_stage_bytes(INT8);
@@ -608,7 +622,7 @@ __global__ void __launch_bounds__(512, 2) dense4_many_kernel(Dense a, const char
     }
 }
 
-// The sums of a result's workgroups, in order of their inputs.
+// The sums of a result's workgroups, in order of their inputs (64 x 4096 of 8: 4.7 us, most of it the launch).
 template <bool INT8>
 __global__ void __launch_bounds__(256) dense4_join_kernel(Dense a, const float *__restrict__ part, const float *__restrict__ back, int splits) {
     const int m = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -710,34 +724,45 @@ inline bool few(size_t M, int K, int N, bool int8) {
     return M <= (int8 ? 64u : 16u) && (int64_t)windows * rounds < 8;
 }
 
+// More tiles of outputs than compute units: two a workgroup, for which the rows are laid out once (2 rows, 5000 x 4096: 7.6 us by one
+// tile, 7.9 by two; 5000 x 5000: 12.8 and 8.0; 8 rows of 8 bits, 16384 x 6144: 16.8 and 14.5).
+constexpr int WIDE = 4096;
+
 // ROWS: the most that there may be.
-template <int G, int DIGITS, int ROWS, int NT, int PF, bool LOOP>
+template <int G, int DIGITS, int ROWS, int NT, int PF, bool LOOP, bool SIDE = false>
 int launch_few(const Dense &a) {
     constexpr int CT = (ROWS * DIGITS + 15) / 16, LAID = DIGITS == 4 && ROWS == 12 ? 16 : ROWS, RPT = PF * LAID < 4 ? 1 : PF * LAID / 4;
     const size_t rows = (size_t)WAVES * PF * 128 * a.M * DIGITS, sums = (size_t)WAVES * NT * CT * 1024, bytes = rows > sums ? rows : sums;
-    hipLaunchKernelGGL((dense4_few_kernel<G, DIGITS, CT, NT, PF, RPT, LOOP>), dim3((a.cols / 16 + NT - 1) / NT), dim3(WAVES * 64), bytes, xsmi::stream(), a);
+    hipLaunchKernelGGL((dense4_few_kernel<G, DIGITS, CT, NT, PF, RPT, LOOP, SIDE>), dim3((a.cols / 16 + NT - 1) / NT), dim3(WAVES * 64), bytes, xsmi::stream(), a);
     XSMI_LAUNCH_CHECK("dense4_few_kernel");
     return XSMI_OK;
+}
+
+// Rows of one tile of columns.
+template <int G, int DIGITS, int ROWS, bool SIDE>
+int launch_tile(const Dense &a, int each) {
+    if (each <= 1) return launch_few<G, DIGITS, ROWS, 1, 1, false, SIDE>(a);
+    if (each <= 2) return launch_few<G, DIGITS, ROWS, 1, 2, false, SIDE>(a);
+    // (one window of two tiles is worth its registers where the scales of 32 inputs do not take twice as many more: 2 rows, 4096 x 16384,
+    // groups of 64: 12.0 us by one tile, 9.4 by two; 3000 x 12000, groups of 32: 10.8 and 13.3)
+    if (each <= 4 && a.cols > WIDE && (SIDE || G != 32)) return launch_few<G, DIGITS, ROWS, 2, 4, false, SIDE>(a);
+    if (each <= 4) return launch_few<G, DIGITS, ROWS, 1, 4, false, SIDE>(a);
+    if (ROWS == 1) return each <= 8 ? launch_few<G, DIGITS, 1, 1, 8, false, SIDE>(a) : launch_few<G, DIGITS, 1, 1, 4, true, SIDE>(a);
+    if (a.cols > WIDE) return launch_few<G, DIGITS, ROWS, 2, 2, true, SIDE>(a);
+    return launch_few<G, DIGITS, ROWS, 1, 4, true, SIDE>(a);
 }
 
 // One window where a wave's chunks fit one, and 64 KB of LDS.
 template <int G, int DIGITS>
 int launch_few(const Dense &a) {
     constexpr int FULL = 16 / DIGITS;                // rows of a tile of columns
+    constexpr int APART = FULL * G / 128;            // and those whose groups find columns side by side
     const int R = a.M * DIGITS, each = (a.chunks + WAVES - 1) / WAVES;
-    if (a.M == 1) {
-        if (each <= 1) return launch_few<G, DIGITS, 1, 1, 1, false>(a);
-        if (each <= 2) return launch_few<G, DIGITS, 1, 1, 2, false>(a);
-        if (each <= 4) return launch_few<G, DIGITS, 1, 1, 4, false>(a);
-        if (each <= 8) return launch_few<G, DIGITS, 1, 1, 8, false>(a);
-        return launch_few<G, DIGITS, 1, 1, 4, true>(a);
+    if (a.M == 1) return launch_tile<G, DIGITS, 1, G != 128>(a, each);
+    if constexpr (G != 128 && APART > 1) {
+        if (a.M <= APART) return launch_tile<G, DIGITS, APART, true>(a, each);
     }
-    if (R <= 16) {
-        if (each <= 1) return launch_few<G, DIGITS, FULL, 1, 1, false>(a);
-        if (each <= 2) return launch_few<G, DIGITS, FULL, 1, 2, false>(a);
-        if (each <= 4) return launch_few<G, DIGITS, FULL, 1, 4, false>(a);
-        return launch_few<G, DIGITS, FULL, 1, 4, true>(a);
-    }
+    if (R <= 16) return launch_tile<G, DIGITS, FULL, false>(a, each);
     if (R <= 32) return launch_few<G, DIGITS, 2 * FULL, 2, 2, true>(a);
     // (three tiles of float32 rows are up to twelve, which lay out as sixteen)
     if (R <= 48) return launch_few<G, DIGITS, 3 * FULL, 2, 1, true>(a);
