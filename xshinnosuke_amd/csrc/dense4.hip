@@ -715,18 +715,19 @@ inline Split split_of(int M, int K, int N) {
     return Split{(pairs + each - 1) / each, each};
 }
 
+// More tiles of outputs than compute units: two a workgroup, for which the rows are laid out once (2 rows, 5000 x 4096: 7.6 us by one
+// tile, 7.9 by two; 5000 x 5000: 12.8 and 8.0; 43 rows of 8 bits, groups of 32, 4096 x 4096: 9.7 and 12.7; 5000 x 7001: 26.1 and 18.3).
+constexpr int WIDE = 4096;
+
 // Few rows: those whose digits fit two tiles of columns, and up to four tiles where a wave goes through less than eight windows: each
-// takes some 3 us then, and the many rows' kernels 12 us and more in all (16 rows, 8192 x 2048: 27.0 us as few, 19.4 as
-// many; 12 rows, 4096 x 4096: 13.5 and 16; 64 rows of 8 bits, 8192 x 8192: 26.2 and 20.3; 43, 5000 x 7001: 18.2 and 20.4).
+// takes some 3 us then, and the many rows' kernels 12 us and more in all (16 rows, 8192 x 2048: 25.6 us as few, 19.9 as
+// many; 12 rows, 4096 x 4096: 12.7 and 16; 43 rows of 8 bits, 5000 x 7001: 18.3 and 20.4).  Three tiles of 8-bit rows with one tile of
+// outputs a workgroup take less for a window (43, 8192 x 4096: 14.2 as few, 18.0 as many; 16384 x 4096: 25.4 and 22.4).
 inline bool few(size_t M, int K, int N, bool int8) {
     if (M <= (int8 ? 32u : 8u)) return true;
     const int windows = (up(K, 128) / 128 + WAVES - 1) / WAVES, rounds = (up(N, 32) / 32 + 255) / 256;
-    return M <= (int8 ? 64u : 16u) && (int64_t)windows * rounds < 8;
+    return M <= (int8 ? 64u : 16u) && (int64_t)windows * rounds < (int8 && M <= 48 && N <= WIDE ? 12 : 8);
 }
-
-// More tiles of outputs than compute units: two a workgroup, for which the rows are laid out once (2 rows, 5000 x 4096: 7.6 us by one
-// tile, 7.9 by two; 5000 x 5000: 12.8 and 8.0; 8 rows of 8 bits, 16384 x 6144: 16.8 and 14.5).
-constexpr int WIDE = 4096;
 
 // ROWS: the most that there may be.
 template <int G, int DIGITS, int ROWS, int NT, int PF, bool LOOP, bool SIDE = false>
@@ -752,6 +753,12 @@ int launch_tile(const Dense &a, int each) {
     return launch_few<G, DIGITS, ROWS, 1, 4, true, SIDE>(a);
 }
 
+// Rows of several tiles of columns.
+template <int G, int DIGITS, int ROWS, int PF>
+int launch_wide(const Dense &a) {
+    return a.cols > WIDE ? launch_few<G, DIGITS, ROWS, 2, PF, true>(a) : launch_few<G, DIGITS, ROWS, 1, PF, true>(a);
+}
+
 // One window where a wave's chunks fit one, and 64 KB of LDS.
 template <int G, int DIGITS>
 int launch_few(const Dense &a) {
@@ -763,10 +770,10 @@ int launch_few(const Dense &a) {
         if (a.M <= APART) return launch_tile<G, DIGITS, APART, true>(a, each);
     }
     if (R <= 16) return launch_tile<G, DIGITS, FULL, false>(a, each);
-    if (R <= 32) return launch_few<G, DIGITS, 2 * FULL, 2, 2, true>(a);
+    if (R <= 32) return launch_wide<G, DIGITS, 2 * FULL, 2>(a);
     // (three tiles of float32 rows are up to twelve, which lay out as sixteen)
-    if (R <= 48) return launch_few<G, DIGITS, 3 * FULL, 2, 1, true>(a);
-    return launch_few<G, DIGITS, 4 * FULL, 2, 1, true>(a);
+    if (R <= 48) return launch_wide<G, DIGITS, 3 * FULL, 1>(a);
+    return launch_wide<G, DIGITS, 4 * FULL, 1>(a);
 }
 
 template <int G, bool INT8>
