@@ -78,6 +78,12 @@ def test_forward_and_backward(rows, cols, residual):
     assert np.all(np.abs(tg.grad.numpy() - want) <= (n + rows / 256 + min(rows, 16384) / 16 + 18) * EPS * most)
 
 
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,cols", [(40003, 13), (20001, 60), (9000, 200), (9001, 300), (6001, 700), (513, 1024), (600, 5000)])
+def test_forward_and_backward_of_many_rows(rows, cols, residual):
+    test_forward_and_backward(rows, cols, residual)
+
+
 @pytest.mark.parametrize("rows,cols", SIZES)
 def test_rows_in_eight_bits(rows, cols):
     rng = np.random.default_rng(rows * 37 + cols)
