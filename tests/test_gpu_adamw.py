@@ -87,6 +87,23 @@ def test_steps_follow_the_definition(bits, shapes):
                 assert np.abs(a - b).max() <= 5 * steps * EPS * t
 
 
+@pytest.mark.parametrize("bits,size", [(32, 8_000_037), (8, 12_900_037)])
+def test_steps_whose_operands_are_streamed(bits, size):
+    test_steps_follow_the_definition(bits, [(777,), (size,)])
+
+
+def test_moments_decoded_in_one_call_equal_those_in_parts():
+    rng = np.random.default_rng(8)
+    blocks = 101_000
+    codes = [be.to_device(rng.integers(0, 256, blocks * 256, dtype=np.uint8)) for _ in range(2)]
+    exponents = [be.to_device(rng.integers(least, 254, blocks, dtype=np.uint8)) for least in (48, 64)]
+    whole = be.kernels.adamw_moments(*codes, *exponents)
+    for a, b in ((0, 50_000), (50_000, blocks)):
+        part = be.kernels.adamw_moments(*[c.leading(256 * a, 256 * b) for c in codes], *[e.leading(a, b) for e in exponents])
+        for x, y in zip(whole, part):
+            assert np.array_equal(x.leading(256 * a, 256 * b).numpy(), y.numpy())
+
+
 def test_extreme_gradients_in_eight_bits():
     """Infinite, NaN, huge and vanishing gradients: a block that held one reads as NaN, the others are not touched."""
     rng = np.random.default_rng(3)

@@ -84,6 +84,11 @@ def test_forward_and_backward_of_many_rows(rows, cols, residual):
     test_forward_and_backward(rows, cols, residual)
 
 
+@pytest.mark.parametrize("rows,cols", [(70_000, 240), (17_000, 1000), (4_100, 4000), (2_100, 8000)])
+def test_forward_and_backward_of_operands_that_are_streamed(rows, cols):
+    test_forward_and_backward(rows, cols, True)
+
+
 @pytest.mark.parametrize("rows,cols", SIZES)
 def test_rows_in_eight_bits(rows, cols):
     rng = np.random.default_rng(rows * 37 + cols)

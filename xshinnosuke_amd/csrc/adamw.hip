@@ -137,8 +137,8 @@ __device__ __forceinline__ void store4(float *p, uint64_t i, uint64_t n, f4 v) {
     if (i + 2 < n) p[i + 2] = v.z;
 }
 
-// 256 threads, four elements each of one tensor: more of them a thread gains nothing (ResNet-18, 11.7 million elements: 57.5 us, 5.7 TB/s;
-// eight a thread 58.2, sixteen 60.3).  The moments are padded to whole blocks of 256 elements, of which those behind the tensor stay
+// 256 threads, four elements each of one tensor: more of them a thread gains nothing (ResNet-18, 11.7 million elements, from the caches: 57.5 us;
+// eight a thread 58.2, sixteen 60.3).  Streamed, from memory: 57 us, 5.7 TB/s; not streamed 62.  The moments are padded to whole blocks of 256 elements, of which those behind the tensor stay
 // zero: zero gradients of zero moments.
 template <bool STREAM>
 __global__ void __launch_bounds__(256) adamw_kernel(Tensors t, float *__restrict__ m, float *__restrict__ v, Factors f,
@@ -312,9 +312,11 @@ int xsmi_adamw_step(int count, float *const *ps, const float *const *gs, const s
     XSMI_LAUNCH_CHECK("adamw_tick_kernel");
     const Factors f = {(float)(1.0 - lr * weight_decay), (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
     const Moments8 q = {(uint8_t *)m, (uint8_t *)v, m_exp, v_exp};
-    double bytes = 0;                                    // read; past the last-level cache (256 MB) they are streamed
+    // What is read: past half of the last-level cache (256 MB) it is streamed, for a forward and a backward have the cache before it comes
+    // again (ResNet-18, 187 MB: 66.5 us without and 58.0 with, after other operands; 51.7 and 56.4 if nothing ran in between).
+    double bytes = 0;
     for (int i = 0; i < count; ++i) bytes += (double)ns[i] * (state_bits == 32 ? 16 : 10);
-    const bool stream = bytes > 256e6;
+    const bool stream = bytes > 128e6;
     for (int done = 0; done < count;) {
         Tensors t;
         uint64_t groups = 0;
