@@ -156,6 +156,34 @@ def test_higher_dimensions_host_tensors_and_recorded_products():
                 be.zeros((999,)).numpy()
 
 
+def test_two_recordings_and_eager_calls_share_a_workspace():
+    rng = np.random.default_rng(11)
+    weight, _ = _weight(rng, 700, 300, 32)
+    inputs = [be.empty((m, 700)) for m in (100, 300, 500)]
+
+    def fill():
+        for a in inputs:
+            a.set(rng.standard_normal(a.shape).astype(np.float32))
+
+    with xs.no_grad():
+        graphs, outs = [], []
+        for a in inputs[:2]:                         # the second recording finds the first one's workspace too small
+            a.set(np.zeros(a.shape, np.float32))
+            graphs.append(xs.StepGraph())
+            with graphs[-1].capture():
+                outs.append(F.dense_4bit(xs.Tensor(a), weight))
+        for turn in range(4):
+            fill()
+            for i in ((0, 1), (1, 0), (0, 1), (1,))[turn]:
+                graphs[i].replay()
+                if turn == 1:                        # a larger one between two replays
+                    F.dense_4bit(xs.Tensor(inputs[2]), weight)
+                recorded = outs[i].numpy()
+                assert np.array_equal(recorded, F.dense_4bit(xs.Tensor(inputs[i]), weight).numpy())
+            if turn == 2:
+                graphs[0].close()
+
+
 def test_a_trained_network_is_served_with_packed_weights(tmp_path):
     """Dense -> norm -> ReLU -> Dense, packed: the logits are those of the dequantised weights; a checkpoint keeps them."""
     np.random.seed(3)
