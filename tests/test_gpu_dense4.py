@@ -68,7 +68,7 @@ def test_products(k, n, group):
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("k,n", [(1500, 4100), (3000, 4130), (5000, 4150)])
+@pytest.mark.parametrize("k,n", [(1500, 4100), (3000, 4130), (5000, 4150), (7500, 4110)])
 def test_products_of_more_tiles_than_compute_units(k, n, group):
     test_products(k, n, group)
 

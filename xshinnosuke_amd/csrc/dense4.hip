@@ -132,7 +132,7 @@ __device__ __forceinline__ void digits8(const int *x, u2 *to) {
 // Columns without a row repeat the last one: a column's sums are its own.  LOOP: there is more than one window.
 // One row, 8192 x 8192, groups of 128: 9.5 us, 3.6 TB/s, a chain of loads, digits, sums and their join; what a wave does between loads is
 // longer than the loads.  SIDE: where rows are so few that all groups of a chunk find columns side by side, each column meets zeros outside of its group, and
-// a chunk's sums are scaled once and not once for each group (one row, 8192 x 16384, groups of 32: 28.7 -> 21.6 us; 8-bit: 26.1 -> 18.2).
+// a chunk's sums are scaled once and not once for each group (one row, 8192 x 16384, groups of 32: 20.0 us, one by one 28.7; 8-bit: 17.0 and 26.1).
 template <int G, int DIGITS, int CT, int NT, int PF, int RPT, bool LOOP, bool SIDE>
 __global__ void __launch_bounds__(WAVES * 64, 2) dense4_few_kernel(Dense a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -748,6 +748,9 @@ int launch_tile(const Dense &a, int each) {
     // groups of 64: 12.0 us by one tile, 9.4 by two; 3000 x 12000, groups of 32: 10.8 and 13.3)
     if (each <= 4 && a.cols > WIDE && (SIDE || G != 32)) return launch_few<G, DIGITS, ROWS, 2, 4, false, SIDE>(a);
     if (each <= 4) return launch_few<G, DIGITS, ROWS, 1, 4, false, SIDE>(a);
+    // (one row of long inputs: the vector unit bounds groups of 32, and two tiles save it the rows' layout; 16384 x 8192: 23.0 us by one tile,
+    // 19.1 by two; groups of 128: 16.6 and 17.9)
+    if (ROWS == 1 && G == 32 && each >= 8 && a.cols > WIDE) return launch_few<G, DIGITS, 1, 2, 2, true, SIDE>(a);
     if (ROWS == 1) return each <= 8 ? launch_few<G, DIGITS, 1, 1, 8, false, SIDE>(a) : launch_few<G, DIGITS, 1, 1, 4, true, SIDE>(a);
     if (a.cols > WIDE) return launch_few<G, DIGITS, ROWS, 2, 2, true, SIDE>(a);
     return launch_few<G, DIGITS, ROWS, 1, 4, true, SIDE>(a);
